@@ -56,7 +56,9 @@ enum sph_status {
   SPH_ERR_TOO_LARGE = 5,
   SPH_ERR_STATIC_SCRATCH_EXCEEDED = 6
 };
-enum sph_dtype { SPH_F32 = 0, SPH_F64 = 1 };
+/* bfloat16 and float16: the norm, log-probability and optimizer entry points at
+ * the end, which take float32 too and no float64. */
+enum sph_dtype { SPH_F32 = 0, SPH_F64 = 1, SPH_BF16 = 2, SPH_F16 = 3 };
 enum sph_interp { SPH_NEAREST = 0, SPH_BILINEAR = 1, SPH_BISPHERICAL = 2 };
 enum sph_precision { SPH_PRECISION_EXACT = 0, SPH_PRECISION_BF16 = 1 };
 
@@ -483,6 +485,82 @@ int sph_mapped_tconv_backward(const void *gout, const void *x, const void *map, 
                               void *gx, void *gw, void *gb, int64_t B, int64_t Cin, int64_t Cout, int64_t IH,
                               int64_t IW, int64_t OH, int64_t OW, int64_t K, int64_t P, int dtype, int interp,
                               int precision, void *ws, size_t ws_bytes, void *stream);
+
+/* ------------------------------------------------------------------------
+ * Operators of the rest of a training or serving step (no counterpart in the
+ * reference, which takes them from its host framework).  dtype: SPH_F32,
+ * SPH_BF16 or SPH_F16; arithmetic, sums and statistics are float32.
+ *
+ * Layouts.  Rows: inner = 1, tensors (outer, C), the rows of x, residual and
+ * s each *_stride elements apart (>= C), outputs and gradients dense.
+ * Planes: inner > 1, tensors (outer, C, inner), dense, strides not read.
+ * outer, C, inner up to 2^31, 2^30, 2^31, outer * inner up to 2^38.
+ *
+ * Root-mean-square norm over C.
+ *   forward   s = residual + x, rounded to dtype and written to `sum` (both
+ *             or neither; without them s = x); rstd = 1/sqrt(mean s^2 + eps);
+ *             out = s * rstd * weight (weight (C), or NULL).  With `scale`
+ *             (float32, one per norm) out is e4m3 and out * scale the value,
+ *             scale = max|s rstd weight| / 448, and 0 over a norm of zeros.
+ *             `rstd` (float32, one per norm) may be NULL.
+ *   backward  gx = rstd (g - u mean(g u)) + gsum with g = gout * weight and
+ *             u = s * rstd, the gradient of x and of residual; gw = sum over
+ *             the norms of gout * u, in a fixed order.  gsum may be NULL; gx
+ *             or gw may be.  gw needs scratch of
+ *             sph_rms_norm_workspace_bytes.
+ * weight_dtype: SPH_F32 or dtype, of weight and gw.
+ * ---------------------------------------------------------------------- */
+int sph_rms_norm_forward(const void *x, const void *residual, const void *weight, void *sum, void *out, float *scale,
+                         float *rstd, int64_t outer, int64_t C, int64_t inner, int64_t x_stride, int64_t r_stride,
+                         double eps, int dtype, int weight_dtype, void *stream);
+size_t sph_rms_norm_workspace_bytes(int64_t outer, int64_t C, int64_t inner);
+int sph_rms_norm_backward(const void *gout, const void *gsum, const void *s, const void *weight, const float *rstd,
+                          void *gx, void *gw, int64_t outer, int64_t C, int64_t inner, int64_t s_stride, int dtype,
+                          int weight_dtype, void *ws, size_t ws_bytes, void *stream);
+
+/* ------------------------------------------------------------------------
+ * Log probabilities over C classes (tokens, or labels of pixels).
+ *   forward   log_probs = log softmax(x)[target], entropy, lse (may be NULL)
+ *             (one float32 per distribution), and the k <= C most probable
+ *             classes, (outer, k, inner): their log probabilities `top` and
+ *             indices `top_index`; equal logits in the order of their indices.
+ *   backward  gx from the gradients g of log_probs, h of entropy (either may
+ *             be NULL; stride 1, or 0: one value for all) and t of top (may
+ *             be NULL).
+ * A target equal to ignore_index has log probability 0 and no gradient; any
+ * other outside [0, C) gives NaN.  Logits of -inf are classes out of the
+ * question; a distribution of nothing else has log probabilities -inf,
+ * entropy 0 and no gradient.
+ * ---------------------------------------------------------------------- */
+int sph_token_log_probs_forward(const void *x, const int64_t *target, float *log_probs, float *entropy, float *lse,
+                                float *top, int64_t *top_index, int64_t outer, int64_t C, int64_t inner,
+                                int64_t x_stride, int64_t k, int64_t ignore_index, int dtype, void *stream);
+int sph_token_log_probs_backward(const void *x, const int64_t *target, const float *lse, const float *entropy,
+                                 const int64_t *top_index, const float *g, int64_t g_stride, const float *h,
+                                 int64_t h_stride, const float *t, void *gx, int64_t outer, int64_t C, int64_t inner,
+                                 int64_t x_stride, int64_t k, int64_t ignore_index, int dtype, void *stream);
+
+/* ------------------------------------------------------------------------
+ * AdamW step over many tensors (HOST arrays of device pointers, read before
+ * the call returns):
+ *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2, with
+ *   g = grad * grad_scale;
+ *   w = w (1 - lr weight_decay) - lr m / (1 - beta1^step)
+ *                                 / (sqrt(v / (1 - beta2^step)) + eps)
+ * dtype of all params, grad_dtype (dtype or SPH_F32) of all grads; with
+ * `masters` (16-bit params only) w is the float32 master and the param its
+ * rounded copy.  state_bits 32: m, v float32.  8: e4m3, with a float32 scale
+ * for each 256 values of a tensor in m_scales, v_scales (ceil(numel / 256)
+ * each); v is held as its square root.  A block of 256 whose values are all
+ * below 2^-100 is held as zeros.  step_at (DEVICE, may be NULL): the step's
+ * number, instead of `step`, and lr_at then, if not NULL, instead of `lr`:
+ * for steps that a CUDA graph replays.
+ * ---------------------------------------------------------------------- */
+int sph_adamw_step(int64_t tensors, void *const *params, const void *const *grads, float *const *masters,
+                   void *const *m, void *const *v, float *const *m_scales, float *const *v_scales,
+                   const int64_t *numels, int dtype, int grad_dtype, int state_bits, double lr, double beta1,
+                   double beta2, double eps, double weight_decay, double grad_scale, double step, const float *lr_at,
+                   const float *step_at, void *stream);
 
 #ifdef __cplusplus
 }

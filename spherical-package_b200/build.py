@@ -23,7 +23,9 @@ OUT = os.path.join(HERE, "_spherical_distortion_ext")
 OBJ = os.path.join(HERE, "build", "obj")
 INCLUDE = os.path.join(ROOT, "include")
 
-CU_SOURCES = ["resample.cu", "plan.cu", "pool.cu", "maps.cu", "conv.cu", "conv_simt.cu", "conv_small.cu", "conv_tc.cu", "conv_x3.cu"]
+CU_SOURCES = ["resample.cu", "plan.cu", "pool.cu", "maps.cu", "conv.cu", "conv_simt.cu", "conv_small.cu", "conv_tc.cu", "conv_x3.cu",
+              "norm.cu", "log_probs.cu", "adamw.cu"]
+SHIM_SOURCES = ["torch_shim.cpp", "torch_shim_net.cpp"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--extended-lambda",
               "-Xcompiler", "-fPIC", "-I" + INCLUDE, "-I" + CSRC]
 # extra compiler flags for developer builds, e.g. SPHMAP_NVCC_FLAGS="-DSPH_TC_TIMING" (per-role cycle counters)
@@ -80,18 +82,27 @@ def build_ext(verbose=False):
     import torch
     from torch.utils import cpp_extension as ce
 
-    src = os.path.join(CSRC, "torch_shim.cpp")
     out = os.path.join(OUT, "_C" + sysconfig.get_config_var("EXT_SUFFIX"))
-    if _newer(out, [src, os.path.join(INCLUDE, "sphmap.h")]):
+    header = os.path.join(INCLUDE, "sphmap.h")
+    if _newer(out, [os.path.join(CSRC, f) for f in SHIM_SOURCES] + [header]):
         return out
     cxx = "/usr/bin/g++" if os.path.exists("/usr/bin/g++") else "g++"
     cuda_home = os.environ.get("CUDA_HOME", "/usr/local/cuda")
-    cmd = [cxx, "-shared", "-fPIC", "-std=c++17", "-O2", "-w", "-DTORCH_EXTENSION_NAME=_C",
-           "-DTORCH_API_INCLUDE_EXTENSION_H", "-D_GLIBCXX_USE_CXX11_ABI=" + str(int(torch._C._GLIBCXX_USE_CXX11_ABI)),
-           "-I" + INCLUDE]
+    flags = ["-fPIC", "-std=c++17", "-O2", "-w", "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
+             "-D_GLIBCXX_USE_CXX11_ABI=" + str(int(torch._C._GLIBCXX_USE_CXX11_ABI)), "-I" + INCLUDE]
     for i in ce.include_paths() + [sysconfig.get_paths()["include"], os.path.join(cuda_home, "include")]:
-        cmd += ["-isystem", i]
-    cmd += [src, "-o", out, "-L" + OUT, "-lsphmap", "-Wl,-rpath,$ORIGIN"]
+        flags += ["-isystem", i]
+    os.makedirs(OBJ, exist_ok=True)
+
+    def one(src):
+        s, o = os.path.join(CSRC, src), os.path.join(OBJ, src[:-4] + ".o")
+        if not _newer(o, [s, header]):
+            _run([cxx] + flags + ["-c", s, "-o", o])
+        return o
+
+    with ThreadPoolExecutor(len(SHIM_SOURCES)) as ex:
+        objs = list(ex.map(one, SHIM_SOURCES))
+    cmd = [cxx, "-shared"] + objs + ["-o", out, "-L" + OUT, "-lsphmap", "-Wl,-rpath,$ORIGIN"]
     for lp in ce.library_paths():
         cmd += ["-L" + lp, "-Wl,-rpath," + lp]
     cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",

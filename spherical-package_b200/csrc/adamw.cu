@@ -1,0 +1,291 @@
+// AdamW step over many tensors in one launch per 'kMaxTensors' of them:
+//
+//     m = b1 m + (1 - b1) g;   v = b2 v + (1 - b2) g^2;
+//     w = w (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// Moments in float32, or in e4m3 with one float32 scale for each 256 values of a tensor: m as it is, v as its square root
+// (e4m3 spans 2^18 between its smallest and largest value, so the root keeps 2^36 of v) with what is positive never held as
+// zero, which would divide m by eps.  Values are rounded to nearest: rounding at random instead would add, every step, a
+// noise that the average over 1 / (1 - b2) steps does not forget (at e4m3's steps and b2 = 0.999 about the size of v itself).
+// What is not finite is held as NaN, and leaves the other values of its 256 as they are.
+#include "element.cuh"
+
+namespace sph {
+
+constexpr int kAdamBlock = 256;  // values behind one scale, and what a warp takes at once: eight a lane
+
+struct AdamTensor {
+  void *param;
+  const void *grad;
+  float *master;
+  void *m, *v;
+  float *m_scale, *v_scale;
+  int64_t n;
+};
+template <int CAP> struct AdamArgs {
+  AdamTensor tensor[CAP];
+  int first[CAP + 1];         // first block of 256 values of each tensor; one past the last behind them
+  unsigned char aligned[CAP];  // four values may be read at once
+  int tensors;
+  float lr, beta1, beta2, rest1, rest2, eps, decay, grad_scale;  // rest = 1 - beta, which 1.f - (float)beta is 5e-5 off
+  double log_beta1, log_beta2;
+  float step_size, root;     // lr / (1 - b1^t), 1 / sqrt(1 - b2^t); from the device's values where there are any
+  const float *lr_at, *step_at;
+};
+
+// Four neighbouring values.
+__device__ __forceinline__ void load4(const float *p, float (&v)[4]) {
+  const float4 q = *(const float4 *)p;
+  v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+}
+template <typename T> __device__ __forceinline__ void load4(const T *p, float (&v)[4]) {
+  union { uint2 u; T t[4]; } q;
+  q.u = *(const uint2 *)p;
+#pragma unroll
+  for (int i = 0; i < 4; i++) v[i] = to_float(q.t[i]);
+}
+__device__ __forceinline__ void store4(float *p, const float (&v)[4]) { *(float4 *)p = make_float4(v[0], v[1], v[2], v[3]); }
+template <typename T> __device__ __forceinline__ void store4(T *p, const float (&v)[4]) {
+  union { uint2 u; T t[4]; } q;
+#pragma unroll
+  for (int i = 0; i < 4; i++) q.t[i] = from_float<T>(v[i]);
+  *(uint2 *)p = q.u;
+}
+struct E4m3 {
+  __nv_fp8_storage_t v;
+};
+__device__ __forceinline__ float to_float(E4m3 v) { return from_e4m3(v.v); }
+__device__ __forceinline__ void load4(const E4m3 *p, float (&v)[4]) {
+  const unsigned q = *(const unsigned *)p;
+#pragma unroll
+  for (int i = 0; i < 4; i++) v[i] = from_e4m3((__nv_fp8_storage_t)(q >> (8 * i)));
+}
+__device__ __forceinline__ void store4(E4m3 *p, const float (&v)[4]) {
+  unsigned q = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) q |= (unsigned)to_e4m3(v[i]) << (8 * i);
+  *(unsigned *)p = q;
+}
+template <> __device__ __forceinline__ E4m3 from_float<E4m3>(float v) { return E4m3{to_e4m3(v)}; }
+
+// A lane's eight of a warp's 256 values: [4 lane, 4 lane + 4) of each half, or every 32nd where four may not be read at once
+// or the tensor ends inside.
+template <typename T> __device__ __forceinline__ void load8(const T *p, int lane, bool four, int n, float (&v)[8]) {
+  if (four) {
+    float a[4], b[4];
+    load4(p + 4 * lane, a);
+    load4(p + 128 + 4 * lane, b);
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = lane + 32 * i < n ? to_float(p[lane + 32 * i]) : 0.f;
+  }
+}
+template <typename T> __device__ __forceinline__ void store8(T *p, int lane, bool four, int n, const float (&v)[8]) {
+  if (four) {
+    const float a[4] = {v[0], v[1], v[2], v[3]}, b[4] = {v[4], v[5], v[6], v[7]};
+    store4(p + 4 * lane, a);
+    store4(p + 128 + 4 * lane, b);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (lane + 32 * i < n) p[lane + 32 * i] = from_float<T>(v[i]);
+  }
+}
+
+__device__ __forceinline__ float finite_max(const float (&v)[8]) {
+  float a = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const float b = fabsf(v[i]);
+    a = b < INFINITY && b > a ? b : a;
+  }
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(a)));
+}
+
+template <typename P, typename G, bool EIGHT, bool MASTER, int CAP>
+__global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ AdamArgs<CAP> a) {
+  const int lane = threadIdx.x & 31, block = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (block >= a.first[a.tensors]) return;
+  int lo = 0, hi = a.tensors;  // the tensor that holds the block: first[lo] <= block < first[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.first[mid] <= block) lo = mid; else hi = mid;
+  }
+  const AdamTensor &t = a.tensor[lo];
+  const int64_t b = block - a.first[lo], at = b * kAdamBlock;
+  const int n = t.n - at < kAdamBlock ? (int)(t.n - at) : kAdamBlock;
+  const bool four = n == kAdamBlock && a.aligned[lo];
+  float lr = a.lr, step_size = a.step_size, root = a.root;
+  if (a.step_at) {
+    if (a.lr_at) lr = *a.lr_at;
+    const double step = (double)*a.step_at;
+    step_size = (float)(lr / -expm1(step * a.log_beta1));
+    root = (float)(1.0 / sqrt(-expm1(step * a.log_beta2)));
+  }
+  float w[8], g[8], m[8], v[8];
+  load8((const G *)t.grad + at, lane, four, n, g);
+  if (MASTER)
+    load8(t.master + at, lane, four, n, w);
+  else
+    load8((const P *)t.param + at, lane, four, n, w);
+  if (EIGHT) {
+    load8((const E4m3 *)t.m + at, lane, four, n, m);
+    load8((const E4m3 *)t.v + at, lane, four, n, v);
+    const float ms = t.m_scale[b], vs = t.v_scale[b];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      m[i] *= ms;
+      v[i] *= vs;
+      v[i] *= v[i];
+    }
+  } else {
+    load8((const float *)t.m + at, lane, four, n, m);
+    load8((const float *)t.v + at, lane, four, n, v);
+  }
+  const float keep = 1.f - lr * a.decay;
+  float u[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const float gi = g[i] * a.grad_scale;
+    m[i] = a.beta1 * m[i] + a.rest1 * gi;
+    v[i] = a.beta2 * v[i] + a.rest2 * gi * gi;
+    u[i] = sqrtf(v[i]);
+    w[i] = w[i] * keep - step_size * (m[i] / (u[i] * root + a.eps));
+  }
+  if (MASTER) store8(t.master + at, lane, four, n, w);
+  store8((P *)t.param + at, lane, four, n, w);
+  if (EIGHT) {
+    const Scale ms = Scale::of(finite_max(m)), us = Scale::of(finite_max(u));
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float p = u[i] * us.inverse;
+      m[i] = fabsf(m[i]) < INFINITY ? m[i] * ms.inverse : NAN;
+      u[i] = !(u[i] < INFINITY) ? NAN : p > 0.f ? fmaxf(p, 0x1p-9f) : p;
+    }
+    store8((E4m3 *)t.m + at, lane, four, n, m);
+    store8((E4m3 *)t.v + at, lane, four, n, u);
+    if (lane == 0) {
+      t.m_scale[b] = ms.scale;
+      t.v_scale[b] = us.scale;
+    }
+  } else {
+    store8((float *)t.m + at, lane, four, n, m);
+    store8((float *)t.v + at, lane, four, n, v);
+  }
+}
+
+inline bool four_aligned(const AdamTensor &t, int param_size, int grad_size, int state_size) {
+  return ((uintptr_t)t.param % (4 * param_size) | (uintptr_t)t.grad % (4 * grad_size) | (uintptr_t)t.m % (4 * state_size) |
+          (uintptr_t)t.v % (4 * state_size) | (uintptr_t)t.master % 16) == 0;
+}
+
+template <typename P, typename G, bool EIGHT, bool MASTER, int CAP>
+void adamw_launch(const AdamArgs<CAP> &a, cudaStream_t st) {
+  adamw_kernel<P, G, EIGHT, MASTER, CAP><<<(unsigned)cdiv(a.first[a.tensors], 8), 256, 0, st>>>(a);
+}
+template <int CAP> void adamw_dispatch(const AdamArgs<CAP> &a, int dtype, int grad_dtype, bool eight, bool master, cudaStream_t st) {
+  SPH_DISPATCH_ELEMENT(dtype, {
+    if (grad_dtype == SPH_F32 || dtype == SPH_F32) {
+      if (eight && master)
+        adamw_launch<T, float, true, true>(a, st);
+      else if (eight)
+        adamw_launch<T, float, true, false>(a, st);
+      else if (master)
+        adamw_launch<T, float, false, true>(a, st);
+      else
+        adamw_launch<T, float, false, false>(a, st);
+    } else {
+      if (eight && master)
+        adamw_launch<T, T, true, true>(a, st);
+      else if (eight)
+        adamw_launch<T, T, true, false>(a, st);
+      else if (master)
+        adamw_launch<T, T, false, true>(a, st);
+      else
+        adamw_launch<T, T, false, false>(a, st);
+    }
+  });
+}
+
+// The tensors [from, to) of a call; kernel parameters hold at most 32,764 bytes.
+constexpr int kFewTensors = 32, kMaxTensors = 440;
+static_assert(sizeof(AdamArgs<kMaxTensors>) <= 32764, "kernel parameters");
+
+}  // namespace sph
+
+using namespace sph;
+
+template <int CAP>
+static int adamw_group(int from, int count, void *const *params, const void *const *grads, float *const *masters, void *const *m,
+                       void *const *v, float *const *m_scales, float *const *v_scales, const int64_t *numels, int dtype, int grad_dtype,
+                       int state_bits, const AdamArgs<1> &common, cudaStream_t st) {
+  AdamArgs<CAP> a;
+  a.tensors = count;
+  a.lr = common.lr, a.beta1 = common.beta1, a.beta2 = common.beta2, a.eps = common.eps, a.decay = common.decay;
+  a.rest1 = common.rest1, a.rest2 = common.rest2, a.grad_scale = common.grad_scale, a.log_beta1 = common.log_beta1, a.log_beta2 = common.log_beta2;
+  a.step_size = common.step_size, a.root = common.root, a.lr_at = common.lr_at, a.step_at = common.step_at;
+  int64_t blocks = 0;
+  for (int i = 0; i < count; i++) {
+    const int k = from + i;
+    a.tensor[i] = AdamTensor{params[k], grads[k], masters ? masters[k] : nullptr, m[k], v[k], m_scales ? m_scales[k] : nullptr,
+                             v_scales ? v_scales[k] : nullptr, numels[k]};
+    a.aligned[i] = four_aligned(a.tensor[i], (int)element_size(dtype), (int)element_size(grad_dtype), state_bits / 8);
+    a.first[i] = (int)blocks;
+    blocks += (numels[k] + kAdamBlock - 1) / kAdamBlock;
+  }
+  a.first[count] = (int)blocks;
+  if (blocks == 0) return 0;
+  adamw_dispatch<CAP>(a, dtype, grad_dtype, state_bits == 8, masters != nullptr, st);
+  return 1;
+}
+
+extern "C" int sph_adamw_step(int64_t tensors, void *const *params, const void *const *grads, float *const *masters, void *const *m,
+                              void *const *v, float *const *m_scales, float *const *v_scales, const int64_t *numels, int dtype,
+                              int grad_dtype, int state_bits, double lr, double beta1, double beta2, double eps, double weight_decay,
+                              double grad_scale, double step, const float *lr_at, const float *step_at, void *stream) {
+  SPH_RANGE("sph_adamw_step");
+  if (!element_dtype(dtype) || !element_dtype(grad_dtype) || (grad_dtype != SPH_F32 && grad_dtype != dtype) ||
+      (state_bits != 8 && state_bits != 32) || (masters && dtype == SPH_F32))
+    return SPH_ERR_UNSUPPORTED;
+  if (tensors < 0 || (tensors > 0 && (!params || !grads || !m || !v || !numels)) || !(beta1 >= 0 && beta1 < 1) ||
+      !(beta2 >= 0 && beta2 < 1) || !(eps >= 0) || (!step_at && !(step >= 1)) || (lr_at && !step_at) ||
+      (state_bits == 8 && tensors > 0 && (!m_scales || !v_scales)))
+    return SPH_ERR_INVALID_ARGUMENT;
+  for (int64_t i = 0; i < tensors; i++) {
+    if (numels[i] < 0 || (numels[i] > 0 && (!params[i] || !grads[i] || !m[i] || !v[i] || (masters && !masters[i]) ||
+                                            (state_bits == 8 && (!m_scales[i] || !v_scales[i])))))
+      return SPH_ERR_INVALID_ARGUMENT;
+    if (numels[i] > ((int64_t)1 << 38)) return SPH_ERR_TOO_LARGE;
+  }
+  AdamArgs<1> c{};
+  c.lr = (float)lr, c.beta1 = (float)beta1, c.beta2 = (float)beta2, c.eps = (float)eps, c.decay = (float)weight_decay;
+  c.rest1 = (float)(1.0 - beta1), c.rest2 = (float)(1.0 - beta2), c.grad_scale = (float)grad_scale;
+  c.log_beta1 = log(beta1), c.log_beta2 = log(beta2);
+  c.lr_at = lr_at, c.step_at = step_at;
+  if (!step_at) {
+    c.step_size = (float)(lr / (1.0 - pow(beta1, step)));
+    c.root = (float)(1.0 / sqrt(1.0 - pow(beta2, step)));
+  }
+  cudaStream_t st = (cudaStream_t)stream;
+  int launches = 0;
+  for (int64_t from = 0; from < tensors;) {
+    // as many tensors as the parameters hold and 2^31 blocks number
+    int count = 0;
+    int64_t blocks = 0;
+    while (from + count < tensors && count < kMaxTensors) {
+      blocks += (numels[from + count] + kAdamBlock - 1) / kAdamBlock;
+      if (blocks > 0x7fffff00ll && count > 0) break;
+      count++;
+    }
+    if (count <= kFewTensors)
+      launches += adamw_group<kFewTensors>((int)from, count, params, grads, masters, m, v, m_scales, v_scales, numels, dtype, grad_dtype,
+                                           state_bits, c, st);
+    else
+      launches += adamw_group<kMaxTensors>((int)from, count, params, grads, masters, m, v, m_scales, v_scales, numels, dtype, grad_dtype,
+                                           state_bits, c, st);
+    from += count;
+  }
+  return launches ? launch_status(launches) : SPH_OK;
+}

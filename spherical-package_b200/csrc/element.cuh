@@ -1,0 +1,84 @@
+// Element types of the operators around the convolutions (norm, log probabilities, optimizer step): float32, bfloat16 and
+// float16 in memory, float32 in registers, one rounding to nearest on the way out; e4m3 for what is held in 8 bits.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace sph {
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+// What a value is once it has been stored as T.
+template <typename T> __device__ __forceinline__ float as_stored(float v) { return to_float(from_float<T>(v)); }
+
+// A weight of its own type, float32 or the data's.
+template <typename T> __device__ __forceinline__ float load_weight(const void *w, int64_t i, bool f32) {
+  return f32 ? __ldg((const float *)w + i) : to_float(((const T *)w)[i]);
+}
+template <typename T> __device__ __forceinline__ void store_weight(void *w, int64_t i, float v, bool f32) {
+  if (f32)
+    ((float *)w)[i] = v;
+  else
+    ((T *)w)[i] = from_float<T>(v);
+}
+
+// Values held in 8 bits: e4m3 times a float32 scale, the largest magnitude of a group at e4m3's largest, 448.  A group
+// whose values all lie below kTiny (448 / amax would not be finite much below it) is a group of zeros with scale 0.
+constexpr float kE4m3Max = 448.f, kTiny = 0x1p-100f;
+struct Scale {
+  float scale, inverse;
+  static __device__ __forceinline__ Scale of(float amax) {
+    const bool zero = amax < kTiny;
+    return Scale{zero ? 0.f : amax / kE4m3Max, zero ? 0.f : kE4m3Max / amax};
+  }
+};
+__device__ __forceinline__ __nv_fp8_storage_t to_e4m3(float v) { return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
+__device__ __forceinline__ float from_e4m3(__nv_fp8_storage_t v) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3)));
+}
+
+// Largest magnitude so far; NaN stays.
+__device__ __forceinline__ float max_nan(float a, float b) { return b > a || b != b ? b : a; }
+
+// Sums (or other joins) over the threads of a warp or of a block; every thread gets the same value.
+template <class F> __device__ __forceinline__ float warp_join(float v, F f) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, d));
+  return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+  return warp_join(v, [](float a, float b) { return a + b; });
+}
+// `shared`: one float per warp.
+template <class F> __device__ __forceinline__ float block_join(float v, float *shared, F f) {
+  v = warp_join(v, f);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  if (lane == 0) shared[warp] = v;
+  __syncthreads();
+  float r = shared[0];
+  for (int i = 1; i < warps; i++) r = f(r, shared[i]);
+  __syncthreads();
+  return r;
+}
+
+// Run a statement with T = the element type of a dtype code.
+#define SPH_DISPATCH_ELEMENT(dtype, ...)                                \
+  switch (dtype) {                                                      \
+    case SPH_BF16: { using T = __nv_bfloat16; __VA_ARGS__; break; }     \
+    case SPH_F16: { using T = __half; __VA_ARGS__; break; }             \
+    default: { using T = float; __VA_ARGS__; break; }                   \
+  }
+inline bool element_dtype(int dtype) { return dtype == SPH_F32 || dtype == SPH_BF16 || dtype == SPH_F16; }
+inline size_t element_size(int dtype) { return dtype == SPH_F32 ? 4 : 2; }
+
+}  // namespace sph

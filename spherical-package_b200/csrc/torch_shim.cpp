@@ -1247,7 +1247,10 @@ OptTensor resample_op(const torch::Tensor &x, const torch::Tensor &map, Interpol
 
 }  // namespace
 
+void bind_network_ops(pybind11::module_ &m);  // torch_shim_net.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  bind_network_ops(m);
   // include/layers/enum_export.h:8-29
   py::enum_<InterpolationType>(m, "InterpolationType", py::arithmetic(), "How a fractional map coordinate is sampled")
       .value("NEAREST", InterpolationType::NEAREST)

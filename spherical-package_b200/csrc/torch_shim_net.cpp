@@ -1,0 +1,462 @@
+// Host side of the operators around the convolutions: root-mean-square norm, log probabilities and the AdamW step, over the C
+// ABI of libsphmap.so.  Part of the extension whose module torch_shim.cpp defines.
+//
+// A tensor is taken as rows (its normalised or classified dimension has stride 1 and the others are one run of equal steps:
+// the last dimension of a contiguous tensor, a slice of wider rows, dimension 1 of a channels-last image) or as planes (a
+// contiguous tensor, any dimension).  Others are refused.
+#include <torch/extension.h>
+
+#include <ATen/TracerMode.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+
+#include <algorithm>
+#include <mutex>
+#include <vector>
+
+#include "sphmap.h"
+
+namespace {
+
+using torch::Tensor;
+using torch::autograd::Node;
+using torch::autograd::SavedVariable;
+using torch::autograd::variable_list;
+using OptTensor = c10::optional<Tensor>;
+
+void ok(int status, const char *what) { TORCH_CHECK(status == SPH_OK, what, ": ", sph_status_string(status)); }
+
+void *current_stream() { return (void *)at::cuda::getCurrentCUDAStream().stream(); }
+
+int element_of(const Tensor &t, const char *name) {
+  switch (t.scalar_type()) {
+    case torch::kFloat: return SPH_F32;
+    case torch::kBFloat16: return SPH_BF16;
+    case torch::kHalf: return SPH_F16;
+    default: TORCH_CHECK(false, name, " must be float32, bfloat16 or float16, got ", t.scalar_type());
+  }
+}
+
+void check_device(const Tensor &t, const char *name, const Tensor &like) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor (this build has no CPU path)");
+  TORCH_CHECK(t.device() == like.device(), name, " must be on the same device as the input");
+}
+
+// How a tensor lies in memory around one of its dimensions.
+struct Layout {
+  int64_t dim, outer, C, inner, stride;  // stride of rows (inner == 1)
+  bool moved;                            // rows whose dimension is not the last: outputs are rows seen through movedim
+};
+
+Layout layout_of(const Tensor &t, int64_t dim, const char *name) {
+  TORCH_CHECK(t.dim() >= 1, name, " must have at least one dimension");
+  TORCH_CHECK(t.layout() == torch::kStrided, name, " must be a dense tensor");
+  TORCH_CHECK(dim >= -t.dim() && dim < t.dim(), "dim must be in [", -t.dim(), ", ", t.dim() - 1, "], got ", dim);
+  Layout l{dim < 0 ? dim + t.dim() : dim, 1, 0, 1, 0, false};
+  l.C = t.size(l.dim);
+  TORCH_CHECK(l.C > 0, name, " must have at least one value along dim");
+  for (int64_t i = 0; i < t.dim(); i++)
+    if (i != l.dim) (i < l.dim ? l.outer : l.inner) *= t.size(i);
+  if (l.outer * l.inner == 0) {  // nothing in it: rows
+    l.outer = 0, l.inner = 1, l.stride = l.C;
+    l.moved = l.dim != t.dim() - 1;
+    return l;
+  }
+  if (t.is_contiguous()) {
+    if (l.inner == 1 || l.C == 1) l.outer *= l.inner, l.inner = 1;
+    l.stride = l.C;
+    return l;
+  }
+  bool rows = l.C == 1 || t.stride(l.dim) == 1;
+  int64_t step = l.C, run = -1;  // the rows' stride (of one row: any), and the one that the next dimension has to have
+  for (int64_t i = t.dim() - 1; i >= 0 && rows; i--) {
+    if (i == l.dim || t.size(i) == 1) continue;
+    if (run < 0) step = t.stride(i);
+    else if (t.stride(i) != run) rows = false;
+    run = t.stride(i) * t.size(i);
+  }
+  TORCH_CHECK(rows && step >= l.C, name, " must be contiguous, or rows of one stride with dim of stride 1");
+  l.outer *= l.inner, l.inner = 1, l.stride = step;
+  l.moved = l.dim != t.dim() - 1;
+  return l;
+}
+
+std::vector<int64_t> sizes_without(const Tensor &t, int64_t dim) {
+  std::vector<int64_t> s = t.sizes().vec();
+  s.erase(s.begin() + dim);
+  return s;
+}
+// A dense tensor of the layout's order with n values along its dimension.
+Tensor like_layout(const Tensor &t, const Layout &l, int64_t n, torch::ScalarType type) {
+  std::vector<int64_t> s = t.sizes().vec();
+  const auto options = t.options().dtype(type).memory_format(c10::nullopt).requires_grad(false);
+  if (!l.moved) {
+    s[l.dim] = n;
+    return torch::empty(s, options);
+  }
+  s = sizes_without(t, l.dim);
+  s.push_back(n);
+  return torch::empty(s, options).movedim(-1, l.dim);
+}
+// Another tensor of the same sizes, dense in that order (copied if it is not).
+Tensor in_layout(const Tensor &t, const Layout &l) {
+  return l.moved ? t.movedim(l.dim, -1).contiguous().movedim(-1, l.dim) : t.contiguous();
+}
+
+bool transformed(std::initializer_list<const Tensor *> ts) {
+  if (at::tracer::impl::is_dispatch_enabled() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode))
+    return true;
+  for (const Tensor *t : ts)
+    if (t != nullptr && t->defined() && t->_fw_grad(0).defined()) return true;
+  return false;
+}
+bool wants_grad(std::initializer_list<const Tensor *> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor *t : ts)
+    if (t != nullptr && t->defined() && t->requires_grad()) return true;
+  return false;
+}
+template <class N> std::shared_ptr<N> new_node(const torch::autograd::edge_list &edges) {
+  std::shared_ptr<N> n(new N(), torch::autograd::deleteNode);
+  n->set_next_edges(torch::autograd::edge_list(edges));
+  return n;
+}
+// Gradients of a backward pass that is to be differentiated itself raise when that happens.
+variable_list once(variable_list r) {
+  if (!at::GradMode::is_enabled()) return r;
+  variable_list some;
+  for (const Tensor &t : r)
+    if (t.defined()) some.push_back(t.detach().requires_grad_());
+  some = (*std::make_shared<torch::autograd::DelayedError>("this operator cannot be differentiated twice", (int64_t)some.size()))(std::move(some));
+  size_t k = 0;
+  for (Tensor &t : r)
+    if (t.defined()) t = some[k++];
+  return r;
+}
+
+// ---- root-mean-square norm -----------------------------------------------------------------------------------------
+struct NormResult {
+  Tensor out, sum, scale, rstd;
+  Layout layout;
+};
+
+NormResult norm_forward(const Tensor &x, const Tensor &weight, const Tensor &residual, double eps, int64_t dim, bool quantized, bool train) {
+  const int dtype = element_of(x, "input");
+  NormResult r;
+  r.layout = layout_of(x, dim, "input");
+  const Layout &l = r.layout;
+  TORCH_CHECK(eps >= 0 && std::isfinite(eps), "eps must be finite and not negative, got ", eps);
+  int64_t r_stride = 0;
+  if (weight.defined()) {
+    TORCH_CHECK(weight.dim() == 1 && weight.size(0) == l.C, "weight must have the size (", l.C, ",) of the normalised dimension");
+    TORCH_CHECK(weight.scalar_type() == torch::kFloat || weight.scalar_type() == x.scalar_type(),
+                "weight must be float32 or have the input's dtype");
+    TORCH_CHECK(weight.is_contiguous(), "weight must be contiguous");
+  }
+  if (residual.defined()) {
+    TORCH_CHECK(residual.sizes() == x.sizes(), "residual must have the input's size");
+    TORCH_CHECK(residual.scalar_type() == x.scalar_type(), "residual must have the input's dtype");
+    const Layout q = layout_of(residual, dim, "residual");
+    TORCH_CHECK(q.inner == l.inner && q.moved == l.moved, "residual must have the input's memory layout");
+    r_stride = q.stride;
+  }
+  check_device(x, "input", x);
+  if (weight.defined()) check_device(weight, "weight", x);
+  if (residual.defined()) check_device(residual, "residual", x);
+  c10::cuda::CUDAGuard guard(x.device());
+  r.out = like_layout(x, l, l.C, quantized ? torch::kFloat8_e4m3fn : x.scalar_type());
+  if (residual.defined()) r.sum = like_layout(x, l, l.C, x.scalar_type());
+  const auto f32 = x.options().dtype(torch::kFloat).memory_format(c10::nullopt).requires_grad(false);
+  if (quantized) r.scale = torch::empty(sizes_without(x, l.dim), f32);
+  if (train) r.rstd = torch::empty({l.outer * l.inner}, f32);
+  ok(sph_rms_norm_forward(x.data_ptr(), residual.defined() ? residual.data_ptr() : nullptr, weight.defined() ? weight.data_ptr() : nullptr,
+                          r.sum.defined() ? r.sum.data_ptr() : nullptr, r.out.data_ptr(),
+                          quantized ? r.scale.data_ptr<float>() : nullptr, train ? r.rstd.data_ptr<float>() : nullptr, l.outer, l.C,
+                          l.inner, l.stride, r_stride, eps, dtype,
+                          weight.defined() && weight.scalar_type() == torch::kFloat ? SPH_F32 : dtype, current_stream()),
+     "sph_rms_norm_forward");
+  return r;
+}
+
+struct RmsNormNode : public Node {
+  SavedVariable s, weight, rstd;
+  bool added = false;  // s is the sum, an output
+  Layout layout;
+  std::mutex mu;
+  std::string name() const override { return "RmsNormBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mu);
+    for (SavedVariable *v : {&s, &weight, &rstd}) v->reset_data();
+  }
+  variable_list apply(variable_list &&g) override {
+    std::lock_guard<std::mutex> lock(mu);
+    variable_list r(3);
+    {
+      at::NoGradGuard no_grad;
+      const Tensor x = added ? s.unpack(shared_from_this()) : s.unpack(), w = weight.unpack(), rs = rstd.unpack();
+      const bool want_x = task_should_compute_output(0) || task_should_compute_output(1), want_w = w.defined() && task_should_compute_output(2);
+      Tensor gout = g[0], gsum = added && g.size() > 1 ? g[1] : Tensor();
+      if (!gout.defined()) gout = torch::zeros_like(x);
+      c10::cuda::CUDAGuard guard(x.device());
+      gout = in_layout(gout, layout);
+      if (gsum.defined()) gsum = in_layout(gsum, layout);
+      const int dtype = element_of(x, "input");
+      const Layout &l = layout;
+      Tensor gx, gw, ws;
+      if (want_x) gx = like_layout(x, l, l.C, x.scalar_type());
+      if (want_w) {
+        gw = torch::empty_like(w);
+        ws = torch::empty({(int64_t)sph_rms_norm_workspace_bytes(l.outer, l.C, l.inner)}, x.options().dtype(torch::kUInt8).memory_format(c10::nullopt));
+      }
+      if (want_x || want_w)
+        ok(sph_rms_norm_backward(gout.data_ptr(), gsum.defined() ? gsum.data_ptr() : nullptr, x.data_ptr(), w.defined() ? w.data_ptr() : nullptr,
+                                 rs.data_ptr<float>(), want_x ? gx.data_ptr() : nullptr, want_w ? gw.data_ptr() : nullptr, l.outer, l.C,
+                                 l.inner, added ? l.C : l.stride, dtype,
+                                 w.defined() && w.scalar_type() == torch::kFloat ? SPH_F32 : dtype, want_w ? ws.data_ptr() : nullptr,
+                                 want_w ? (size_t)ws.numel() : 0, current_stream()),
+           "sph_rms_norm_backward");
+      if (task_should_compute_output(0)) r[0] = gx;
+      if (task_should_compute_output(1)) r[1] = gx;
+      if (want_w) r[2] = gw;
+    }
+    return once(std::move(r));
+  }
+};
+
+// (out,) or (out, sum); nothing where the native node is invisible to what looks at the call.
+c10::optional<std::vector<Tensor>> rms_norm(const Tensor &x, const OptTensor &weight, const OptTensor &residual, double eps, int64_t dim,
+                                            bool inside) {
+  const Tensor w = weight.value_or(Tensor()), res = residual.value_or(Tensor());
+  if (!inside && transformed({&x, &w, &res})) return c10::nullopt;
+  const bool train = wants_grad({&x, &w, &res});
+  NormResult r;
+  {
+    at::NoGradGuard no_grad;
+    r = norm_forward(x, w, res, eps, dim, false, train);
+  }
+  std::vector<Tensor> out{r.out};
+  if (res.defined()) out.push_back(r.sum);
+  if (train) {
+    auto n = new_node<RmsNormNode>(torch::autograd::collect_next_edges(x, res, w));
+    n->layout = r.layout;
+    n->added = res.defined();
+    torch::autograd::set_history(out, n);
+    n->s = n->added ? SavedVariable(out[1], true) : SavedVariable(x, false);
+    n->weight = SavedVariable(w, false);
+    n->rstd = SavedVariable(r.rstd, false);
+  }
+  return out;
+}
+
+std::vector<Tensor> rms_norm_quantized(const Tensor &x, const OptTensor &weight, const OptTensor &residual, double eps, int64_t dim) {
+  at::NoGradGuard no_grad;
+  NormResult r = norm_forward(x, weight.value_or(Tensor()), residual.value_or(Tensor()), eps, dim, true, false);
+  std::vector<Tensor> out{r.out, r.scale};
+  if (residual) out.push_back(r.sum);
+  return out;
+}
+
+// ---- log probabilities -----------------------------------------------------------------------------------------------
+struct LogProbsNode : public Node {
+  SavedVariable x, target, lse, entropy, top_index;
+  Layout layout;
+  int64_t k = 0, ignore_index = 0;
+  std::mutex mu;
+  std::string name() const override { return "TokenLogProbsBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mu);
+    for (SavedVariable *v : {&x, &target, &lse, &entropy, &top_index}) v->reset_data();
+  }
+  // One value for all (the gradient of a sum or a mean) is taken as such.
+  static const float *spread(Tensor &g, int64_t &stride) {
+    stride = 1;
+    if (!g.defined()) return nullptr;
+    bool one = true;
+    for (int64_t i = 0; i < g.dim(); i++) one = one && (g.size(i) == 1 || g.stride(i) == 0);
+    if (one)
+      stride = 0;
+    else
+      g = g.contiguous();
+    return g.data_ptr<float>();
+  }
+  variable_list apply(variable_list &&g) override {
+    std::lock_guard<std::mutex> lock(mu);
+    variable_list r(1);
+    {
+      at::NoGradGuard no_grad;
+      const Tensor in = x.unpack(), t = target.unpack(), s = lse.unpack(), e = entropy.unpack(shared_from_this()), index = top_index.unpack();
+      if (!task_should_compute_output(0)) return r;
+      const Layout &l = layout;
+      c10::cuda::CUDAGuard guard(in.device());
+      r[0] = like_layout(in, l, l.C, in.scalar_type());
+      int64_t g_stride, h_stride;
+      const float *gp = spread(g[0], g_stride), *hp = spread(g[1], h_stride);
+      Tensor gt = k > 0 && g.size() > 2 ? g[2] : Tensor();
+      if (gt.defined()) gt = in_layout(gt, l);
+      ok(sph_token_log_probs_backward(in.data_ptr(), t.data_ptr<int64_t>(), s.data_ptr<float>(), e.data_ptr<float>(),
+                                      gt.defined() ? index.data_ptr<int64_t>() : nullptr, gp, g_stride, hp, h_stride,
+                                      gt.defined() ? gt.data_ptr<float>() : nullptr, r[0].data_ptr(), l.outer, l.C, l.inner, l.stride, k,
+                                      ignore_index, element_of(in, "logits"), current_stream()),
+         "sph_token_log_probs_backward");
+    }
+    return once(std::move(r));
+  }
+};
+
+// (log_probs, entropy[, top_log_probs, top_indices])
+c10::optional<std::vector<Tensor>> token_log_probs(const Tensor &x, const Tensor &target, int64_t dim, int64_t k, int64_t ignore_index,
+                                                   bool inside) {
+  if (!inside && transformed({&x})) return c10::nullopt;
+  const int dtype = element_of(x, "logits");
+  const Layout l = layout_of(x, dim, "logits");
+  TORCH_CHECK(target.scalar_type() == torch::kLong, "target must be int64, got ", target.scalar_type());
+  TORCH_CHECK(target.sizes() == sizes_without(x, l.dim), "target must have the logits' size without dim");
+  TORCH_CHECK(target.is_contiguous(), "target must be contiguous");
+  TORCH_CHECK(k >= 0 && k <= l.C, "top_k must be in [0, ", l.C, "], got ", k);
+  check_device(x, "logits", x);
+  check_device(target, "target", x);
+  const bool train = wants_grad({&x});
+  std::vector<Tensor> out;
+  Tensor lse, index;
+  {
+    at::NoGradGuard no_grad;
+    c10::cuda::CUDAGuard guard(x.device());
+    const auto f32 = x.options().dtype(torch::kFloat).memory_format(c10::nullopt).requires_grad(false);
+    out = {torch::empty(target.sizes(), f32), torch::empty(target.sizes(), f32)};
+    if (k > 0) {
+      out.push_back(like_layout(x, l, k, torch::kFloat));
+      index = like_layout(x, l, k, torch::kLong);
+    }
+    if (train) lse = torch::empty(target.sizes(), f32);
+    ok(sph_token_log_probs_forward(x.data_ptr(), target.data_ptr<int64_t>(), out[0].data_ptr<float>(), out[1].data_ptr<float>(),
+                                   train ? lse.data_ptr<float>() : nullptr, k > 0 ? out[2].data_ptr<float>() : nullptr,
+                                   k > 0 ? index.data_ptr<int64_t>() : nullptr, l.outer, l.C, l.inner, l.stride, k, ignore_index, dtype,
+                                   current_stream()),
+       "sph_token_log_probs_forward");
+  }
+  if (train) {
+    auto n = new_node<LogProbsNode>(torch::autograd::collect_next_edges(x));
+    n->layout = l;
+    n->k = k;
+    n->ignore_index = ignore_index;
+    torch::autograd::set_history(out, n);
+    n->x = SavedVariable(x, false);
+    n->target = SavedVariable(target, false);
+    n->lse = SavedVariable(lse, false);
+    n->entropy = SavedVariable(out[1], true);
+    n->top_index = SavedVariable(index, false);
+  }
+  if (k > 0) out.push_back(index);
+  return out;
+}
+
+// ---- AdamW -----------------------------------------------------------------------------------------------------------
+using Tensors = std::vector<Tensor>;
+using OptTensors = c10::optional<std::vector<OptTensor>>;
+
+void adamw_step(const Tensors &params, const Tensors &grads, const Tensors &m, const Tensors &v, const OptTensors &masters,
+                const c10::optional<Tensors> &m_scales, const c10::optional<Tensors> &v_scales, double step, double lr, double beta1,
+                double beta2, double eps, double weight_decay, double grad_scale, const OptTensor &step_at, const OptTensor &lr_at) {
+  const size_t n = params.size();
+  TORCH_CHECK(grads.size() == n && m.size() == n && v.size() == n && (!masters || masters->size() == n) &&
+                  (!m_scales || m_scales->size() == n) && (!v_scales || v_scales->size() == n),
+              "adamw_step: the lists must have the same length");
+  TORCH_CHECK(m_scales.has_value() == v_scales.has_value(), "adamw_step: both moments have scales, or neither");
+  TORCH_CHECK(lr >= 0 && std::isfinite(lr) && weight_decay >= 0 && eps >= 0, "adamw_step: lr, weight_decay and eps must not be negative");
+  TORCH_CHECK(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, "adamw_step: betas must be in [0, 1)");
+  TORCH_CHECK(step_at || step >= 1, "adamw_step: step counts from 1");
+  TORCH_CHECK(!lr_at || step_at, "adamw_step: lr on the device needs step there too");
+  if (n == 0) return;
+  const bool eight = m_scales.has_value();
+  const auto state = eight ? torch::kFloat8_e4m3fn : torch::kFloat;
+  struct Group {
+    int dtype, grad_dtype;
+    bool master;
+    std::vector<void *> p, m, v;
+    std::vector<const void *> g;
+    std::vector<float *> w, ms, vs;
+    std::vector<int64_t> n;
+  };
+  std::vector<Group> groups;
+  std::vector<const void *> seen;
+  seen.reserve(n);
+  for (size_t i = 0; i < n; i++) {
+    const Tensor &p = params[i], &g = grads[i];
+    const int dtype = element_of(p, "param"), grad_dtype = element_of(g, "grad");
+    const bool master = masters && (*masters)[i].has_value();
+    TORCH_CHECK(grad_dtype == dtype || grad_dtype == SPH_F32, "grad must be float32 or have its param's dtype");
+    TORCH_CHECK(!master || dtype != SPH_F32, "a float32 param takes no master");
+    const int64_t blocks = (p.numel() + 255) / 256;
+    const auto fits = [&](const Tensor &t, const char *name, torch::ScalarType type, int64_t numel) {
+      TORCH_CHECK(t.scalar_type() == type, name, " must be ", type, ", got ", t.scalar_type());
+      TORCH_CHECK(t.numel() == numel, name, " must have ", numel, " values, got ", t.numel());
+      TORCH_CHECK(t.layout() == torch::kStrided && t.is_contiguous(), name, " must be contiguous");
+    };
+    fits(p, "param", p.scalar_type(), p.numel());
+    fits(g, "grad", g.scalar_type(), p.numel());
+    fits(m[i], "exp_avg", state, p.numel());
+    fits(v[i], "exp_avg_sq", state, p.numel());
+    if (master) fits(*(*masters)[i], "master", torch::kFloat, p.numel());
+    if (eight) {
+      fits((*m_scales)[i], "exp_avg_scale", torch::kFloat, blocks);
+      fits((*v_scales)[i], "exp_avg_sq_scale", torch::kFloat, blocks);
+    }
+    for (const Tensor *t : {&p, &g, &m[i], &v[i]}) check_device(*t, "every tensor of adamw_step", params[0]);
+    if (master) check_device(*(*masters)[i], "master", params[0]);
+    if (eight)
+      for (const Tensor *t : {&(*m_scales)[i], &(*v_scales)[i]}) check_device(*t, "scale", params[0]);
+    if (p.numel() == 0) continue;
+    seen.push_back(p.data_ptr());
+    size_t at = 0;
+    while (at < groups.size() && !(groups[at].dtype == dtype && groups[at].grad_dtype == grad_dtype && groups[at].master == master)) at++;
+    if (at == groups.size()) {
+      groups.emplace_back();
+      groups[at].dtype = dtype, groups[at].grad_dtype = grad_dtype, groups[at].master = master;
+    }
+    Group &q = groups[at];
+    q.p.push_back(p.data_ptr()), q.g.push_back(g.data_ptr()), q.m.push_back(m[i].data_ptr()), q.v.push_back(v[i].data_ptr());
+    q.n.push_back(p.numel());
+    if (master) q.w.push_back((*masters)[i]->data_ptr<float>());
+    if (eight) q.ms.push_back((*m_scales)[i].data_ptr<float>()), q.vs.push_back((*v_scales)[i].data_ptr<float>());
+  }
+  std::sort(seen.begin(), seen.end());
+  TORCH_CHECK(std::adjacent_find(seen.begin(), seen.end()) == seen.end(), "adamw_step: a param appears twice");
+  const auto scalar = [&](const OptTensor &t, const char *name) -> const float * {
+    if (!t) return nullptr;
+    TORCH_CHECK(t->scalar_type() == torch::kFloat && t->numel() == 1, name, " must be one float32 value");
+    check_device(*t, name, params[0]);
+    return t->data_ptr<float>();
+  };
+  const float *step_p = scalar(step_at, "step"), *lr_p = scalar(lr_at, "lr");
+  c10::cuda::CUDAGuard guard(params[0].device());
+  for (Group &q : groups)
+    ok(sph_adamw_step((int64_t)q.n.size(), q.p.data(), q.g.data(), q.master ? q.w.data() : nullptr, q.m.data(), q.v.data(),
+                      eight ? q.ms.data() : nullptr, eight ? q.vs.data() : nullptr, q.n.data(), q.dtype, q.grad_dtype, eight ? 8 : 32, lr,
+                      beta1, beta2, eps, weight_decay, grad_scale, step, lr_p, step_p, current_stream()),
+       "sph_adamw_step");
+  // written behind autograd's back: whoever saved one of these tensors has to notice
+  const auto touched = [](const Tensor &t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  };
+  for (size_t i = 0; i < n; i++) {
+    touched(params[i]), touched(m[i]), touched(v[i]);
+    if (masters && (*masters)[i]) touched(*(*masters)[i]);
+    if (eight) touched((*m_scales)[i]), touched((*v_scales)[i]);
+  }
+}
+
+}  // namespace
+
+void bind_network_ops(pybind11::module_ &m) {
+  namespace py = pybind11;
+  m.def("rms_norm_op", &rms_norm, py::arg("x"), py::arg("weight"), py::arg("residual"), py::arg("eps"), py::arg("dim"),
+        py::arg("inside") = false);
+  m.def("rms_norm_quantized", &rms_norm_quantized, py::arg("x"), py::arg("weight"), py::arg("residual"), py::arg("eps"), py::arg("dim"));
+  m.def("token_log_probs_op", &token_log_probs, py::arg("x"), py::arg("target"), py::arg("dim"), py::arg("top_k"),
+        py::arg("ignore_index"), py::arg("inside") = false);
+  m.def("adamw_step", &adamw_step, py::arg("params"), py::arg("grads"), py::arg("exp_avgs"), py::arg("exp_avg_sqs"), py::arg("masters"),
+        py::arg("exp_avg_scales"), py::arg("exp_avg_sq_scales"), py::arg("step"), py::arg("lr"), py::arg("beta1"), py::arg("beta2"),
+        py::arg("eps"), py::arg("weight_decay"), py::arg("grad_scale"), py::arg("step_at"), py::arg("lr_at"));
+}

@@ -5,7 +5,12 @@ layers/functional/mapped_pooling.py:203-245, layers/functional/resample.py:113-2
 layers/functional/convolution.py:62-71 and the map-driven halves of
 layers/functional/tangent_images.py:6-55 of the reference: the same call
 signatures and assertions, on top of ``_spherical_distortion_ext``.
+
+Beside them stand operators that a network of mapped convolutions is trained and read with and that the reference takes from
+its host framework: ``rms_norm`` / ``rms_norm_quantized`` and ``token_log_probs`` (the optimizer step is in ``sphmap.optim``).
 """
+from typing import NamedTuple, Optional
+
 import torch
 
 import _spherical_distortion_ext._C as _C
@@ -36,15 +41,17 @@ class _AsFunction(torch.autograd.Function):
             out = op(*inner, True)
         if out is None:
             raise AssertionError("arguments do not fit the operator")
-        many = isinstance(out, tuple)
-        ctx.wanted, ctx.inputs, ctx.output = wanted, [inner[i] for i in wanted], out[0] if many else out
-        result = [o.detach() for o in (out if many else (out,))]
+        many = isinstance(out, (tuple, list))
+        outs = out if many else (out,)
+        ctx.wanted, ctx.inputs, ctx.outputs = wanted, [inner[i] for i in wanted], outs
+        result = [o.detach() for o in outs]
         ctx.mark_non_differentiable(*[o for o in result if not o.is_floating_point()])
         return tuple(result) if many else result[0]
 
     @staticmethod
-    def backward(ctx, grad_output, *_):
-        grads = iter(torch.autograd.grad(ctx.output, ctx.inputs, grad_output, retain_graph=True, allow_unused=True))
+    def backward(ctx, *grad_outputs):
+        pairs = [(o, g) for o, g in zip(ctx.outputs, grad_outputs) if o.requires_grad and g is not None]
+        grads = iter(torch.autograd.grad([o for o, _ in pairs], ctx.inputs, [g for _, g in pairs], retain_graph=True, allow_unused=True))
         return (None,) + tuple(next(grads) if i in ctx.wanted else None for i in range(len(ctx.needs_input_grad) - 1))
 
 
@@ -269,3 +276,51 @@ def convolution(input, weight, bias, kernel_size, stride, padding, dilation):
 
 def transposed_convolution(input, weight, bias, kernel_size, stride, padding, dilation):
     return _TransposedConvolution.apply(input, weight, bias, kernel_size, stride, padding, dilation)
+
+
+# ---- normalisation and log probabilities (no counterpart in the reference) ---------------------------------------
+def rms_norm(input, weight=None, residual=None, eps=1e-6, dim=1):
+    """out = s / sqrt(mean(s^2) + eps) * weight with the mean over `dim` (default: the channels of an image batch) and
+    s = residual + input, or the input alone.  Returns out, or (out, s) with a residual; both are differentiable.
+
+    float32, bfloat16 or float16; statistics are float32.  s is rounded to that type, as it is returned, before it is
+    normalised.  weight (size of dim; float32 or the input's dtype) may be None.  The input is contiguous, or its `dim` has
+    stride 1 and its other dimensions are rows of one stride (a slice of wider rows, a channels-last image); the residual lies
+    alike.  Squares are summed in float32: magnitudes above 1e18 overflow."""
+    args = (input, weight, residual, float(eps), int(dim))
+    out = _C.rms_norm_op(*args)
+    if out is None:
+        out = _by_function(_C.rms_norm_op, args)
+    return out[0] if residual is None else tuple(out)
+
+
+def rms_norm_quantized(input, weight=None, residual=None, eps=1e-6, dim=1):
+    """rms_norm with its output in 8 bits: (q, scale), or (q, scale, s) with a residual, where q is float8_e4m3fn and
+    q * scale.unsqueeze(dim) the output; scale (float32, the input's size without dim) is the largest magnitude of each
+    normalised row / 448, and 0 over a row of zeros.  Forward only (no autograd node)."""
+    return tuple(_C.rms_norm_quantized(input, weight, residual, float(eps), int(dim)))
+
+
+class TokenLogProbs(NamedTuple):
+    log_probs: torch.Tensor
+    entropy: torch.Tensor
+    top_log_probs: Optional[torch.Tensor]
+    top_indices: Optional[torch.Tensor]
+
+
+def token_log_probs(logits, target, dim=1, top_k=0, ignore_index=-100):
+    """Log probabilities of given classes, over `dim` (default: the channels of an image batch, one label per pixel; -1 for
+    rows of tokens), with the entropy of each distribution and its `top_k` most probable classes.
+
+    logits float32, bfloat16 or float16, laid out as for `rms_norm`; target int64, their size without dim.  Results are float32:
+    log_probs and entropy of target's size, top_log_probs and (int64) top_indices with top_k in the place of dim, equal
+    logits in the order of their indices; None with top_k = 0.  All but the indices are differentiable.
+
+    A target equal to ignore_index gives log probability 0 and no gradient, any other outside the classes NaN.  Logits of
+    -inf are classes out of the question; where there is no other, log probabilities are -inf, the entropy 0 and the
+    gradient 0.  +inf and NaN give NaN."""
+    args = (logits, target, int(dim), int(top_k), int(ignore_index))
+    out = _C.token_log_probs_op(*args)
+    if out is None:
+        out = _by_function(_C.token_log_probs_op, args)
+    return TokenLogProbs(*out) if top_k else TokenLogProbs(*out, None, None)

@@ -117,6 +117,30 @@ class MappedAvgUnpool(nn.Module):
         return F.mapped_avg_unpool(x, oh, ow, sample_map, self.kernel_size, self.interp, interp_weights)
 
 
+class RMSNorm(nn.Module):
+    """Root-mean-square norm over the channels (an extension; `dim` -1 for rows of tokens).  With a residual the layer adds it
+    first and returns (out, sum)."""
+
+    def __init__(self, channels, eps=1e-6, dim=1):
+        super().__init__()
+        self.channels, self.eps, self.dim = channels, eps, dim
+        self.weight = nn.Parameter(torch.ones(channels))
+
+    def forward(self, x, residual=None):
+        return F.rms_norm(x, self.weight, residual, self.eps, self.dim)
+
+
+class TokenLogProbs(nn.Module):
+    """Log probabilities of given classes, entropies and the most probable classes (an extension): F.token_log_probs."""
+
+    def __init__(self, dim=1, top_k=0, ignore_index=-100):
+        super().__init__()
+        self.dim, self.top_k, self.ignore_index = dim, top_k, ignore_index
+
+    def forward(self, logits, target):
+        return F.token_log_probs(logits, target, self.dim, self.top_k, self.ignore_index)
+
+
 class ResampleFromUV(nn.Module):
     """Gathers an image from N textures: x (B, C, N, TH, TW), quad_idx (H, W) int64, tex_uv (H, W, 2)."""
 

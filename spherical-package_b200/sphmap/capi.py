@@ -33,6 +33,8 @@ SYMBOLS = [
     "sph_voting_resample_to_map", "sph_map_locality", "sph_build_kernel_map", "sph_build_is_checked", "sph_conv_companion_bytes",
     "sph_staging_bytes", "sph_conv_workspace_preferred_bytes", "sph_resample_from_map_ws", "sph_resample_to_map_ws", "sph_mapped_pool_ws", "sph_mapped_max_unpool_ws",
     "sph_conv_companion_channels", "sph_conv_companion_fill", "sph_trace_phases", "sph_mapped_conv_forward_cl", "sph_mapped_conv_backward_cl", "sph_mapped_tconv_backward",
+    "sph_rms_norm_forward", "sph_rms_norm_workspace_bytes", "sph_rms_norm_backward", "sph_token_log_probs_forward",
+    "sph_token_log_probs_backward", "sph_adamw_step",
 ]
 ERR_UNSUPPORTED = 2
 
@@ -47,6 +49,7 @@ lib.sph_launch_count.restype = ctypes.c_ulonglong
 lib.sph_conv_workspace_bytes.restype = ctypes.c_size_t
 lib.sph_conv_workspace_preferred_bytes.restype = ctypes.c_size_t
 lib.sph_conv_companion_bytes.restype = ctypes.c_size_t
+lib.sph_rms_norm_workspace_bytes.restype = ctypes.c_size_t
 
 _vp, _i64, _int, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t
 
