@@ -24,69 +24,71 @@ struct AdamTensor {
 };
 template <int CAP> struct AdamArgs {
   AdamTensor tensor[CAP];
-  int first[CAP + 1];         // first block of 256 values of each tensor; one past the last behind them
-  unsigned char aligned[CAP];  // four values may be read at once
-  int tensors;
+  int first[CAP + 1];          // first task of each tensor; one past the last behind them
+  unsigned char aligned[CAP];  // eight values may be read at once
+  int tensors, chunk;          // a task: up to chunk blocks of 256 values
   float lr, beta1, beta2, rest1, rest2, eps, decay, grad_scale;  // rest = 1 - beta, which 1.f - (float)beta is 5e-5 off
   double log_beta1, log_beta2;
   float step_size, root;     // lr / (1 - b1^t), 1 / sqrt(1 - b2^t); from the device's values where there are any
   const float *lr_at, *step_at;
 };
 
-// Four neighbouring values.
-__device__ __forceinline__ void load4(const float *p, float (&v)[4]) {
-  const float4 q = *(const float4 *)p;
-  v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+// A lane's eight neighbouring values, in loads and stores of up to 32 bytes.
+__device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
+  asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "l"(p));
 }
-template <typename T> __device__ __forceinline__ void load4(const T *p, float (&v)[4]) {
-  union { uint2 u; T t[4]; } q;
-  q.u = *(const uint2 *)p;
-#pragma unroll
-  for (int i = 0; i < 4; i++) v[i] = to_float(q.t[i]);
+__device__ __forceinline__ void store8(float *p, const float (&v)[8]) {
+  asm volatile("st.global.v8.f32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),
+               "f"(v[5]), "f"(v[6]), "f"(v[7]), "l"(p)
+               : "memory");
 }
-__device__ __forceinline__ void store4(float *p, const float (&v)[4]) { *(float4 *)p = make_float4(v[0], v[1], v[2], v[3]); }
-template <typename T> __device__ __forceinline__ void store4(T *p, const float (&v)[4]) {
-  union { uint2 u; T t[4]; } q;
+template <typename T> __device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
+  union { uint4 u; T t[8]; } q;
+  q.u = *(const uint4 *)p;
 #pragma unroll
-  for (int i = 0; i < 4; i++) q.t[i] = from_float<T>(v[i]);
-  *(uint2 *)p = q.u;
+  for (int i = 0; i < 8; i++) v[i] = to_float(q.t[i]);
+}
+template <typename T> __device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
+  union { uint4 u; T t[8]; } q;
+#pragma unroll
+  for (int i = 0; i < 8; i++) q.t[i] = from_float<T>(v[i]);
+  *(uint4 *)p = q.u;
 }
 struct E4m3 {
   __nv_fp8_storage_t v;
 };
 __device__ __forceinline__ float to_float(E4m3 v) { return from_e4m3(v.v); }
-__device__ __forceinline__ void load4(const E4m3 *p, float (&v)[4]) {
-  const unsigned q = *(const unsigned *)p;
-#pragma unroll
-  for (int i = 0; i < 4; i++) v[i] = from_e4m3((__nv_fp8_storage_t)(q >> (8 * i)));
-}
-__device__ __forceinline__ void store4(E4m3 *p, const float (&v)[4]) {
-  unsigned q = 0;
-#pragma unroll
-  for (int i = 0; i < 4; i++) q |= (unsigned)to_e4m3(v[i]) << (8 * i);
-  *(unsigned *)p = q;
-}
 template <> __device__ __forceinline__ E4m3 from_float<E4m3>(float v) { return E4m3{to_e4m3(v)}; }
-
-// A lane's eight of a warp's 256 values: [4 lane, 4 lane + 4) of each half, or every 32nd where four may not be read at once
-// or the tensor ends inside.
-template <typename T> __device__ __forceinline__ void load8(const T *p, int lane, bool four, int n, float (&v)[8]) {
-  if (four) {
-    float a[4], b[4];
-    load4(p + 4 * lane, a);
-    load4(p + 128 + 4 * lane, b);
+__device__ __forceinline__ void load8(const E4m3 *p, float (&v)[8]) {
+  const uint2 q = *(const uint2 *)p;
 #pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
+  for (int i = 0; i < 4; i++) {
+    const unsigned two = ((i < 2 ? q.x : q.y) >> (16 * (i & 1))) & 0xffffu;
+    const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3)));
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void store8(E4m3 *p, const float (&v)[8]) {
+  unsigned q[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) q[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+  *(uint2 *)p = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+}
+
+// A lane's eight of a warp's 256 values: neighbours, or every 32nd where the tensor is not aligned for that or ends inside.
+template <typename T> __device__ __forceinline__ void load_lane(const T *p, int lane, bool wide, int n, float (&v)[8]) {
+  if (wide) {
+    load8(p + 8 * lane, v);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] = lane + 32 * i < n ? to_float(p[lane + 32 * i]) : 0.f;
   }
 }
-template <typename T> __device__ __forceinline__ void store8(T *p, int lane, bool four, int n, const float (&v)[8]) {
-  if (four) {
-    const float a[4] = {v[0], v[1], v[2], v[3]}, b[4] = {v[4], v[5], v[6], v[7]};
-    store4(p + 4 * lane, a);
-    store4(p + 128 + 4 * lane, b);
+template <typename T> __device__ __forceinline__ void store_lane(T *p, int lane, bool wide, int n, const float (&v)[8]) {
+  if (wide) {
+    store8(p + 8 * lane, v);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; i++)
@@ -94,29 +96,42 @@ template <typename T> __device__ __forceinline__ void store8(T *p, int lane, boo
   }
 }
 
-__device__ __forceinline__ float finite_max(const float (&v)[8]) {
-  float a = 0.f;
+// Codes and scale of a warp's 256 values.
+__device__ __forceinline__ float encode(float (&v)[8], bool root) {
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(v[i]));  // (NaN is passed over, and its code is NaN)
+  amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
+  if (amax == INFINITY) {  // infinities become NaN and leave the others alone
+    amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      v[i] = fabsf(v[i]) < INFINITY ? v[i] : NAN;
+      amax = fmaxf(amax, fabsf(v[i]));
+    }
+    amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
+  }
+  const Scale s = Scale::of(amax);
 #pragma unroll
   for (int i = 0; i < 8; i++) {
-    const float b = fabsf(v[i]);
-    a = b < INFINITY && b > a ? b : a;
+    v[i] *= s.inverse;
+    if (root) v[i] = v[i] > 0.f ? fmaxf(v[i], 0x1p-9f) : v[i];
   }
-  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(a)));
+  return s.scale;
 }
 
+// A warp takes up to `chunk` blocks of 256 values of one tensor.
 template <typename P, typename G, bool EIGHT, bool MASTER, int CAP>
 __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ AdamArgs<CAP> a) {
-  const int lane = threadIdx.x & 31, block = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (block >= a.first[a.tensors]) return;
-  int lo = 0, hi = a.tensors;  // the tensor that holds the block: first[lo] <= block < first[hi]
+  const int lane = threadIdx.x & 31, task = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (task >= a.first[a.tensors]) return;
+  int lo = 0, hi = a.tensors;  // the tensor that holds the task: first[lo] <= task < first[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (a.first[mid] <= block) lo = mid; else hi = mid;
+    if (a.first[mid] <= task) lo = mid; else hi = mid;
   }
   const AdamTensor &t = a.tensor[lo];
-  const int64_t b = block - a.first[lo], at = b * kAdamBlock;
-  const int n = t.n - at < kAdamBlock ? (int)(t.n - at) : kAdamBlock;
-  const bool four = n == kAdamBlock && a.aligned[lo];
+  const bool aligned = a.aligned[lo];
   float lr = a.lr, step_size = a.step_size, root = a.root;
   if (a.step_at) {
     if (a.lr_at) lr = *a.lr_at;
@@ -124,61 +139,63 @@ __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Adam
     step_size = (float)(lr / -expm1(step * a.log_beta1));
     root = (float)(1.0 / sqrt(-expm1(step * a.log_beta2)));
   }
-  float w[8], g[8], m[8], v[8];
-  load8((const G *)t.grad + at, lane, four, n, g);
-  if (MASTER)
-    load8(t.master + at, lane, four, n, w);
-  else
-    load8((const P *)t.param + at, lane, four, n, w);
-  if (EIGHT) {
-    load8((const E4m3 *)t.m + at, lane, four, n, m);
-    load8((const E4m3 *)t.v + at, lane, four, n, v);
-    const float ms = t.m_scale[b], vs = t.v_scale[b];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      m[i] *= ms;
-      v[i] *= vs;
-      v[i] *= v[i];
-    }
-  } else {
-    load8((const float *)t.m + at, lane, four, n, m);
-    load8((const float *)t.v + at, lane, four, n, v);
-  }
   const float keep = 1.f - lr * a.decay;
-  float u[8];
+  int64_t b = (int64_t)(task - a.first[lo]) * a.chunk;
+  for (int j = 0; j < a.chunk; j++, b++) {
+    const int64_t at = b * kAdamBlock;
+    if (at >= t.n) return;
+    const int n = t.n - at < kAdamBlock ? (int)(t.n - at) : kAdamBlock;
+    const bool wide = n == kAdamBlock && aligned;
+    float w[8], g[8], m[8], v[8], u[8];
+    load_lane((const G *)t.grad + at, lane, wide, n, g);
+    if (MASTER)
+      load_lane(t.master + at, lane, wide, n, w);
+    else
+      load_lane((const P *)t.param + at, lane, wide, n, w);
+    if (EIGHT) {
+      load_lane((const E4m3 *)t.m + at, lane, wide, n, m);
+      load_lane((const E4m3 *)t.v + at, lane, wide, n, v);
+      const float ms = t.m_scale[b], vs = t.v_scale[b];
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const float gi = g[i] * a.grad_scale;
-    m[i] = a.beta1 * m[i] + a.rest1 * gi;
-    v[i] = a.beta2 * v[i] + a.rest2 * gi * gi;
-    u[i] = sqrtf(v[i]);
-    w[i] = w[i] * keep - step_size * (m[i] / (u[i] * root + a.eps));
-  }
-  if (MASTER) store8(t.master + at, lane, four, n, w);
-  store8((P *)t.param + at, lane, four, n, w);
-  if (EIGHT) {
-    const Scale ms = Scale::of(finite_max(m)), us = Scale::of(finite_max(u));
+      for (int i = 0; i < 8; i++) {
+        m[i] *= ms;
+        v[i] *= vs;
+        v[i] *= v[i];
+      }
+    } else {
+      load_lane((const float *)t.m + at, lane, wide, n, m);
+      load_lane((const float *)t.v + at, lane, wide, n, v);
+    }
+    // The old moment's product and the root are rounded by themselves, the new term is fused: codes are cut from these
+    // values, and would otherwise depend on what the compiler fuses.
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const float p = u[i] * us.inverse;
-      m[i] = fabsf(m[i]) < INFINITY ? m[i] * ms.inverse : NAN;
-      u[i] = !(u[i] < INFINITY) ? NAN : p > 0.f ? fmaxf(p, 0x1p-9f) : p;
+      const float gi = g[i] * a.grad_scale;
+      m[i] = fmaf(a.rest1, gi, __fmul_rn(a.beta1, m[i]));
+      v[i] = fmaf(__fmul_rn(a.rest2, gi), gi, __fmul_rn(a.beta2, v[i]));
+      u[i] = sqrtf(v[i]);
+      w[i] = fmaf(-step_size, __fdividef(m[i], fmaf(u[i], root, a.eps)), w[i] * keep);
     }
-    store8((E4m3 *)t.m + at, lane, four, n, m);
-    store8((E4m3 *)t.v + at, lane, four, n, u);
-    if (lane == 0) {
-      t.m_scale[b] = ms.scale;
-      t.v_scale[b] = us.scale;
+    if (MASTER) store_lane(t.master + at, lane, wide, n, w);
+    store_lane((P *)t.param + at, lane, wide, n, w);
+    if (EIGHT) {
+      const float ms = encode(m, false), us = encode(u, true);
+      store_lane((E4m3 *)t.m + at, lane, wide, n, m);
+      store_lane((E4m3 *)t.v + at, lane, wide, n, u);
+      if (lane == 0) {
+        t.m_scale[b] = ms;
+        t.v_scale[b] = us;
+      }
+    } else {
+      store_lane((float *)t.m + at, lane, wide, n, m);
+      store_lane((float *)t.v + at, lane, wide, n, v);
     }
-  } else {
-    store8((float *)t.m + at, lane, four, n, m);
-    store8((float *)t.v + at, lane, four, n, v);
   }
 }
 
-inline bool four_aligned(const AdamTensor &t, int param_size, int grad_size, int state_size) {
-  return ((uintptr_t)t.param % (4 * param_size) | (uintptr_t)t.grad % (4 * grad_size) | (uintptr_t)t.m % (4 * state_size) |
-          (uintptr_t)t.v % (4 * state_size) | (uintptr_t)t.master % 16) == 0;
+inline bool wide_aligned(const AdamTensor &t, int param_size, int grad_size, int state_size) {
+  return ((uintptr_t)t.param % (8 * param_size) | (uintptr_t)t.grad % (8 * grad_size) | (uintptr_t)t.m % (8 * state_size) |
+          (uintptr_t)t.v % (8 * state_size) | (uintptr_t)t.master % 32) == 0;
 }
 
 template <typename P, typename G, bool EIGHT, bool MASTER, int CAP>
@@ -227,16 +244,20 @@ static int adamw_group(int from, int count, void *const *params, const void *con
   a.rest1 = common.rest1, a.rest2 = common.rest2, a.grad_scale = common.grad_scale, a.log_beta1 = common.log_beta1, a.log_beta2 = common.log_beta2;
   a.step_size = common.step_size, a.root = common.root, a.lr_at = common.lr_at, a.step_at = common.step_at;
   int64_t blocks = 0;
+  for (int i = 0; i < count; i++) blocks += (numels[from + i] + kAdamBlock - 1) / kAdamBlock;
+  // A warp finds its tensor once for four blocks, where there are enough of those for every SM's 64 warps twice over.
+  a.chunk = blocks >= 148 * 64 * 8 ? 4 : 1;
+  int64_t tasks = 0;
   for (int i = 0; i < count; i++) {
     const int k = from + i;
     a.tensor[i] = AdamTensor{params[k], grads[k], masters ? masters[k] : nullptr, m[k], v[k], m_scales ? m_scales[k] : nullptr,
                              v_scales ? v_scales[k] : nullptr, numels[k]};
-    a.aligned[i] = four_aligned(a.tensor[i], (int)element_size(dtype), (int)element_size(grad_dtype), state_bits / 8);
-    a.first[i] = (int)blocks;
-    blocks += (numels[k] + kAdamBlock - 1) / kAdamBlock;
+    a.aligned[i] = wide_aligned(a.tensor[i], (int)element_size(dtype), (int)element_size(grad_dtype), state_bits / 8);
+    a.first[i] = (int)tasks;
+    tasks += (numels[k] + kAdamBlock * a.chunk - 1) / (kAdamBlock * a.chunk);
   }
-  a.first[count] = (int)blocks;
-  if (blocks == 0) return 0;
+  a.first[count] = (int)tasks;
+  if (tasks == 0) return 0;
   adamw_dispatch<CAP>(a, dtype, grad_dtype, state_bits == 8, masters != nullptr, st);
   return 1;
 }
