@@ -520,8 +520,9 @@ int sph_rms_norm_backward(const void *gout, const void *gsum, const void *s, con
 
 /* ------------------------------------------------------------------------
  * Log probabilities over C classes (tokens, or labels of pixels).
- *   forward   log_probs = log softmax(x)[target], entropy, lse (may be NULL)
- *             (one float32 per distribution), and the k <= C most probable
+ *   forward   log_probs = log softmax(x)[target] and entropy (one float32 per
+ *             distribution), stats (two, for backward; may be NULL: the
+ *             maximum m and sum e^(x - m)), and the k <= C most probable
  *             classes, (outer, k, inner): their log probabilities `top` and
  *             indices `top_index`; equal logits in the order of their indices.
  *   backward  gx from the gradients g of log_probs, h of entropy (either may
@@ -532,10 +533,10 @@ int sph_rms_norm_backward(const void *gout, const void *gsum, const void *s, con
  * question; a distribution of nothing else has log probabilities -inf,
  * entropy 0 and no gradient.
  * ---------------------------------------------------------------------- */
-int sph_token_log_probs_forward(const void *x, const int64_t *target, float *log_probs, float *entropy, float *lse,
+int sph_token_log_probs_forward(const void *x, const int64_t *target, float *log_probs, float *entropy, float *stats,
                                 float *top, int64_t *top_index, int64_t outer, int64_t C, int64_t inner,
                                 int64_t x_stride, int64_t k, int64_t ignore_index, int dtype, void *stream);
-int sph_token_log_probs_backward(const void *x, const int64_t *target, const float *lse, const float *entropy,
+int sph_token_log_probs_backward(const void *x, const int64_t *target, const float *stats, const float *entropy,
                                  const int64_t *top_index, const float *g, int64_t g_stride, const float *h,
                                  int64_t h_stride, const float *t, void *gx, int64_t outer, int64_t C, int64_t inner,
                                  int64_t x_stride, int64_t k, int64_t ignore_index, int dtype, void *stream);

@@ -12,100 +12,388 @@
 // probability 0 and no gradient; other targets outside [0, C) NaN.  Equal logits are ordered by their index, NaN before numbers.
 #include "element.cuh"
 
+#include <cooperative_groups.h>
+
 namespace sph {
+
+namespace cg = cooperative_groups;
 
 struct LogProbArgs {
   const void *x;
   const int64_t *target;
-  float *log_probs, *entropy, *lse, *top;  // top (outer, k, inner)
+  float *log_probs, *entropy, *top;  // top (outer, k, inner)
+  float2 *stats;                     // (m, S) of each distribution, for the backward pass
   int64_t *top_index;
   int64_t outer, inner, x_stride, ignore_index;
   int C, k;
 };
 
-// Order of the candidates as one number: larger is better; value first (NaN above all), then the lower index.
-__device__ __forceinline__ unsigned long long candidate(float v, int index) {
-  unsigned u = __float_as_uint(v + 0.f);  // (-0 and 0 are equal)
-  u = v != v ? 0xffffffffu : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-  return ((unsigned long long)u << 32) | (0xffffffffu - (unsigned)index);
-}
-__device__ __forceinline__ int candidate_index(unsigned long long c) { return (int)(0xffffffffu - (unsigned)c); }
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// Running softmax statistics of a part of a distribution.
+// max that keeps NaN.
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// 2^d for d <= 0 (or NaN), 0 far below.
+__device__ __forceinline__ float exp2_fast(float d) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  return r;
+}
+// log2 e times a logit's distance from the maximum; what is infinitely far below stops at a finite distance whose exponential
+// is 0, so that 0 times it is 0.
+__device__ __forceinline__ float distance(float x, float base) { return fmax_nan((x - base) * kLog2e, -1000.f); }
+
+// Order of the candidates as one number: larger is better; value first (NaN above all), then the lower index.
+__device__ __forceinline__ unsigned order_of(float v) {
+  const unsigned u = __float_as_uint(v + 0.f);  // (-0 and 0 are equal)
+  return v != v ? 0xffffffffu : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(unsigned order) {
+  return order == 0xffffffffu ? NAN : __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
+}
+using Candidate = unsigned long long;
+__device__ __forceinline__ Candidate candidate(unsigned order, int index) {
+  return ((Candidate)order << 32) | (0xffffffffu - (unsigned)index);
+}
+__device__ __forceinline__ int candidate_index(Candidate c) { return (int)(0xffffffffu - (unsigned)c); }
+
+// Softmax statistics of a part of a distribution: its maximum, and with d = (x - m) log2 e the sums of 2^d and of 2^d d.
 struct Stats {
   float m = -INFINITY, s = 0.f, t = 0.f;
-  __device__ __forceinline__ void add(float x) {
-    const float n = fmaxf(m, x), base = n == -INFINITY ? 0.f : n;
-    rescale(base);
-    m = n;
-    const float d = x - base, e = expf(d);
-    s += e;
-    t += e * fmaxf(d, -1e4f);
+  __device__ __forceinline__ float4 packed() const { return make_float4(m, s, t, 0.f); }
+  static __device__ __forceinline__ Stats of(float4 v) {
+    Stats r;
+    r.m = v.x, r.s = v.y, r.t = v.z;
+    return r;
   }
-  // The sums for the maximum `base` instead of m: e^(x-b) = e^(x-m) e^(m-b), and t's terms move by m - b.
-  __device__ __forceinline__ void rescale(float base) {
-    const float d = m - base;
-    if (d == 0.f || m == -INFINITY) return;  // (nothing but -inf so far: the sums are 0, or NaN)
-    const float f = expf(d);
-    t = (t + s * fmaxf(d, -1e4f)) * f;
+  // The maximum that distances are measured from: a finite one while there is nothing but -inf.
+  static __device__ __forceinline__ float base(float m) { return m == -INFINITY ? 0.f : m; }
+  // The sums for another, not smaller maximum: 2^d' = 2^d 2^c and 2^d' d' = (2^d d + 2^d c) 2^c with c = (m - n) log2 e.
+  __device__ __forceinline__ void move_to(float n) {
+    if (m == n) return;
+    const float c = distance(m, base(n)), f = exp2_fast(c);
+    t = fmaf(s, c, t) * f;
     s *= f;
+    m = n;
+  }
+  __device__ __forceinline__ void add(float x) {
+    move_to(fmax_nan(m, x));
+    const float d = distance(x, base(m)), e = exp2_fast(d);
+    s += e;
+    t = fmaf(e, d, t);
   }
   __device__ __forceinline__ void join(Stats o) {
-    const float n = fmaxf(m, o.m), base = n == -INFINITY ? 0.f : n;
-    rescale(base);
-    o.rescale(base);
-    m = n;
+    const float n = fmax_nan(m, o.m);
+    move_to(n);
+    o.move_to(n);
     s += o.s;
     t += o.t;
   }
-  __device__ __forceinline__ float lse() const { return s == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + logf(s); }
+  // Over the warp, the same in every lane.
+  __device__ __forceinline__ void join_warp() {
+    float n = m;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) n = fmax_nan(n, __shfl_xor_sync(0xffffffffu, n, d));
+    move_to(n);
+    s = warp_sum(s);
+    t = warp_sum(t);
+  }
   __device__ __forceinline__ float entropy() const {
-    const float h = s == 0.f ? 0.f : logf(s) - t / s;
+    const float h = s == 0.f ? 0.f : logf(s) - kLn2 * (t / s);
     return h < 0.f ? 0.f : h;
+  }
+  __device__ __forceinline__ float log_prob(float x) const { return s == 0.f ? -INFINITY : (x - m) - logf(s); }
+};
+
+__device__ __forceinline__ void write_stats(const LogProbArgs &a, int64_t at, const Stats &st, int64_t t, float x_t) {
+  a.log_probs[at] = t == a.ignore_index ? 0.f : t < 0 || t >= a.C ? NAN : st.log_prob(x_t);
+  a.entropy[at] = st.entropy();
+  if (a.stats) a.stats[at] = make_float2(Stats::base(st.m), st.s);
+}
+
+// ---- rows ------------------------------------------------------------------------------------------------------------
+// 16 bytes of a row at a time.  A row need not start on a 16-byte boundary: vector v holds the elements [v n - shift, v n - shift + n)
+// with `shift` the elements between the boundary before the row and its start; the vectors at its two ends are put together
+// from single elements.
+template <typename T> struct RowVector {
+  static constexpr int N = 16 / (int)sizeof(T);
+  union {
+    uint4 u;
+    T t[N];
+  };
+  static __device__ __forceinline__ int shift_of(const T *row) { return (int)((uintptr_t)row % 16 / sizeof(T)); }
+  // Elements outside the row are `outside`.
+  __device__ __forceinline__ void load(const T *row, int first, int C, T outside) {
+    if (first >= 0 && first + N <= C) {
+      u = *(const uint4 *)(row + first);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i++) t[i] = first + i >= 0 && first + i < C ? row[first + i] : outside;
+    }
+  }
+  __device__ __forceinline__ void store(T *row, int first, int C) const {
+    if (first >= 0 && first + N <= C) {
+      *(uint4 *)(row + first) = u;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i++)
+        if (first + i >= 0 && first + i < C) row[first + i] = t[i];
+    }
+  }
+  __device__ __forceinline__ float at(int i) const { return to_float(t[i]); }
+};
+
+// A thread's part of a tile: 32 logits in registers.
+template <typename T> struct Tile {
+  static constexpr int N = RowVector<T>::N, V = 32 / N;
+  RowVector<T> v[V];
+  // The vectors at, at + step, ... below `end`; the others are -inf.
+  __device__ __forceinline__ void load(const T *row, int at, int step, int end, int shift, int C) {
+    const T none = from_float<T>(-INFINITY);
+#pragma unroll
+    for (int i = 0; i < V; i++) v[i].load(row, at + i * step < end ? (at + i * step) * N - shift : C, C, none);
+  }
+  __device__ __forceinline__ float largest() const {
+    float m = v[0].at(0);
+#pragma unroll
+    for (int i = 0; i < V; i++)
+#pragma unroll
+      for (int j = 0; j < N; j++) m = fmax_nan(m, v[i].at(j));
+    return m;
+  }
+  __device__ __forceinline__ void add_to(Stats &st, float largest) const {
+    st.move_to(fmax_nan(st.m, largest));
+    const float base = Stats::base(st.m);
+    float s[2] = {0.f, 0.f}, t[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < V; i++)
+#pragma unroll
+      for (int j = 0; j < N; j++) {
+        const float d = distance(v[i].at(j), base), e = exp2_fast(d);
+        s[j & 1] += e;
+        t[j & 1] = fmaf(e, d, t[j & 1]);
+      }
+    st.s += s[0] + s[1];
+    st.t += t[0] + t[1];
+  }
+  // f(order, index) for each logit of order `least` or better.
+  template <class F> __device__ __forceinline__ void each(unsigned least, int at, int step, int end, int shift, int C, F f) const {
+#pragma unroll
+    for (int i = 0; i < V; i++)
+#pragma unroll
+      for (int j = 0; j < N; j++) {
+        const unsigned o = order_of(v[i].at(j));
+        const int index = (at + i * step) * N - shift + j;
+        if (o >= least && at + i * step < end && index >= 0 && index < C) f(o, index);
+      }
   }
 };
 
-__device__ __forceinline__ float target_log_prob(const LogProbArgs &a, int64_t t, float lse, float x_t) {
-  if (t == a.ignore_index) return 0.f;
-  if (t < 0 || t >= a.C) return NAN;
-  return lse == -INFINITY ? -INFINITY : x_t - lse;
+// The k best of n candidates in shared memory, by counting for each how many are better (they are all different).
+__device__ __forceinline__ void rank_candidates(const Candidate *from, int n, int k, Candidate *best) {
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const Candidate mine = from[i];
+    int rank = 0;
+    for (int j = 0; j < n; j++) rank += from[j] > mine;
+    if (rank < k) best[rank] = mine;
+  }
 }
 
-template <typename T> __global__ void __launch_bounds__(256) log_probs_rows_kernel(LogProbArgs a) {
-  __shared__ Stats stats[8];
-  __shared__ unsigned long long best[8];
+constexpr int kRowThreads = 256, kRowTile = kRowThreads * 32, kMostTop = 32, kMostCandidates = 1024, kMostCluster = 16;
+
+// A row belongs to a cluster of blocks (gridDim.x of them, one where there are rows enough); a block walks its run of vectors in
+// tiles of 8192 logits held in registers, each read once.  Of each tile the best are found without looking at most of it: the k-th
+// largest of the maxima of 32 groups of threads is a bound that k logits reach and few others do.
+template <typename T, bool TOP> __global__ void __launch_bounds__(kRowThreads, TOP ? 3 : 4) log_probs_rows_kernel(LogProbArgs a) {
+  __shared__ float4 stats[8], whole;
+  __shared__ unsigned group_best[32];
+  __shared__ Candidate best[2][kMostTop];
+  __shared__ Candidate pool[TOP ? kMostCandidates : 1];
+  __shared__ int pooled;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = (int)gridDim.x, part = (int)blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
+  if (row >= a.outer) return;  // (the whole cluster)
+  const T *x = (const T *)a.x + row * a.x_stride;
+  const int shift = RowVector<T>::shift_of(x), vectors = (int)(((int64_t)a.C + shift + RowVector<T>::N - 1) / RowVector<T>::N);
+  const int per = (vectors + blocks - 1) / blocks, from = min(part * per, vectors), end = min(from + per, vectors);
+  Stats st;
+  int have = 0, now = 0;  // candidates kept so far, in best[now]
+  for (int v0 = from; v0 < end; v0 += kRowThreads * Tile<T>::V) {
+    Tile<T> tile;
+    const int at = v0 + threadIdx.x;
+    tile.load(x, at, kRowThreads, end, shift, a.C);
+    const float largest = tile.largest();
+    if (TOP) {
+      const unsigned mine = order_of(largest);
+      unsigned o = mine;
+#pragma unroll
+      for (int d = 4; d > 0; d >>= 1) o = max(o, __shfl_xor_sync(0xffffffffu, o, d));
+      if ((lane & 7) == 0) group_best[threadIdx.x >> 3] = o;
+      if (threadIdx.x < have) pool[threadIdx.x] = best[now][threadIdx.x];
+      if (threadIdx.x == 0) pooled = have;
+      __syncthreads();
+      o = group_best[lane];
+      unsigned least = 0;
+      for (int i = 0; i < a.k; i++) {  // the k-th largest of the groups' best
+        least = __reduce_max_sync(0xffffffffu, o);
+        const unsigned who = __ballot_sync(0xffffffffu, o == least);
+        if (lane == __ffs(who) - 1) o = 0;
+      }
+      const Candidate worst = have == a.k ? best[now][a.k - 1] : 0;
+      least = max(least, (unsigned)(worst >> 32));
+      if (mine >= least)
+        tile.each(least, at, kRowThreads, end, shift, a.C, [&](unsigned order, int index) {
+          const Candidate c = candidate(order, index);
+          if (c > worst) {
+            const int to = atomicAdd(&pooled, 1);
+            if (to < kMostCandidates) pool[to] = c;
+          }
+        });
+      __syncthreads();
+      const int n = pooled;
+      if (n <= kMostCandidates) {
+        rank_candidates(pool, n, a.k, best[now ^ 1]);
+        have = min(n, a.k);
+      } else {  // very many alike: one after the other, each the best below the last
+        Candidate last = ~0ull;
+        for (int i = 0; i < a.k; i++) {
+          Candidate c = 0;
+          if (threadIdx.x < have && best[now][threadIdx.x] < last) c = best[now][threadIdx.x];
+          tile.each(0, at, kRowThreads, end, shift, a.C, [&](unsigned order, int index) {
+            const Candidate q = candidate(order, index);
+            if (q < last && q > c) c = q;
+          });
+#pragma unroll
+          for (int d = 16; d > 0; d >>= 1) {
+            const Candidate o2 = __shfl_xor_sync(0xffffffffu, c, d);
+            c = o2 > c ? o2 : c;
+          }
+          __syncthreads();
+          if (lane == 0) pool[warp] = c;
+          __syncthreads();
+          c = pool[0];
+          for (int w = 1; w < 8; w++) c = pool[w] > c ? pool[w] : c;
+          last = c;
+          if (threadIdx.x == 0) best[now ^ 1][i] = c;
+        }
+        have = a.k;
+      }
+      now ^= 1;
+      __syncthreads();
+    }
+    tile.add_to(st, largest);
+  }
+  st.join_warp();
+  if (lane == 0) stats[warp] = st.packed();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 8; i++) st.join(Stats::of(stats[i]));
+    whole = st.packed();
+    pooled = have;
+    if (TOP && now == 1)
+      for (int i = 0; i < have; i++) best[0][i] = best[1][i];
+  }
+  if (blocks == 1) {
+    __syncthreads();
+  } else {
+    cluster.sync();
+    if (part == 0) {
+      // a thread per candidate of the others' lists; the first thread of all joins the statistics
+      if (TOP) {
+        int n = 0;
+        for (int b = 0; b < blocks; b++) {
+          const int more = *cluster.map_shared_rank(&pooled, b);
+          for (int i = threadIdx.x; i < more; i += kRowThreads) pool[n + i] = cluster.map_shared_rank(&best[0][0], b)[i];
+          n += more;
+        }
+        __syncthreads();
+        rank_candidates(pool, n, a.k, best[1]);
+      }
+      if (threadIdx.x == 0) {
+        for (int b = 1; b < blocks; b++) st.join(Stats::of(*cluster.map_shared_rank(&whole, b)));
+        whole = st.packed();
+      }
+      __syncthreads();
+    }
+    cluster.sync();  // what was read of the others has to last until here
+    if (part != 0) return;
+    now = 1;
+  }
+  if (threadIdx.x == 0) {
+    const int64_t t = a.target[row];
+    write_stats(a, row, Stats::of(whole), t, t >= 0 && t < a.C ? to_float(x[t]) : 0.f);
+  }
+  if (TOP && threadIdx.x < a.k) {
+    const Candidate c = best[blocks == 1 ? 0 : 1][threadIdx.x];
+    a.top_index[row * a.k + threadIdx.x] = candidate_index(c);
+    a.top[row * a.k + threadIdx.x] = Stats::of(whole).log_prob(value_of((unsigned)(c >> 32)));
+  }
+}
+
+// Rows of up to 1024 classes: a warp each, their logits in registers.
+template <typename T, bool TOP> __global__ void __launch_bounds__(256, TOP ? 2 : 4) log_probs_warp_kernel(LogProbArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= a.outer) return;
+  const T *x = (const T *)a.x + row * a.x_stride;
+  const int shift = RowVector<T>::shift_of(x), vectors = (a.C + shift + RowVector<T>::N - 1) / RowVector<T>::N;
+  Tile<T> tile;
+  tile.load(x, lane, 32, vectors, shift, a.C);
+  const int64_t t = a.target[row];
+  const float x_t = t >= 0 && t < a.C ? to_float(x[t]) : 0.f;
+  Stats st;
+  tile.add_to(st, tile.largest());
+  st.join_warp();
+  if (lane == 0) write_stats(a, row, st, t, x_t);
+  if (!TOP) return;
+  Candidate last = ~0ull;
+  for (int i = 0; i < a.k; i++) {  // the best below the last
+    Candidate c = 0;
+    tile.each(0, lane, 32, vectors, shift, a.C, [&](unsigned order, int index) {
+      const Candidate q = candidate(order, index);
+      if (q < last && q > c) c = q;
+    });
+    const unsigned order = __reduce_max_sync(0xffffffffu, (unsigned)(c >> 32));
+    const unsigned index = __reduce_max_sync(0xffffffffu, (unsigned)(c >> 32) == order ? (unsigned)c : 0u);
+    last = (Candidate)order << 32 | index;
+    if (lane == 0) {
+      a.top_index[row * a.k + i] = candidate_index(last);
+      a.top[row * a.k + i] = st.log_prob(value_of(order));
+    }
+  }
+}
+
+// More of the best than the kernels above keep, after one of them: each pass over the row finds the best below the last.
+template <typename T> __global__ void __launch_bounds__(256) log_probs_many_kernel(LogProbArgs a) {
+  __shared__ Candidate best[8];
+  __shared__ float4 stats[8];
   const int64_t row = blockIdx.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const T *x = (const T *)a.x + row * a.x_stride;
   Stats st;
   for (int c = threadIdx.x; c < a.C; c += 256) st.add(to_float(x[c]));
-  for (int d = 16; d > 0; d >>= 1) {
-    Stats o;
-    o.m = __shfl_xor_sync(0xffffffffu, st.m, d);
-    o.s = __shfl_xor_sync(0xffffffffu, st.s, d);
-    o.t = __shfl_xor_sync(0xffffffffu, st.t, d);
-    st.join(o);
-  }
-  if (lane == 0) stats[warp] = st;
+  st.join_warp();
+  if (lane == 0) stats[warp] = st.packed();
   __syncthreads();
-  st = stats[0];
-  for (int i = 1; i < 8; i++) st.join(stats[i]);
-  const float lse = st.lse();
+  st = Stats::of(stats[0]);
+  for (int i = 1; i < 8; i++) st.join(Stats::of(stats[i]));
   if (threadIdx.x == 0) {
     const int64_t t = a.target[row];
-    a.log_probs[row] = target_log_prob(a, t, lse, t >= 0 && t < a.C ? to_float(x[t]) : 0.f);
-    a.entropy[row] = st.entropy();
-    if (a.lse) a.lse[row] = lse;
+    write_stats(a, row, st, t, t >= 0 && t < a.C ? to_float(x[t]) : 0.f);
   }
-  unsigned long long last = ~0ull;
-  for (int i = 0; i < a.k; i++) {  // the best that comes after the last one
-    unsigned long long mine = 0;
+  Candidate last = ~0ull;
+  for (int i = 0; i < a.k; i++) {
+    Candidate mine = 0;
     for (int c = threadIdx.x; c < a.C; c += 256) {
-      const unsigned long long q = candidate(to_float(x[c]), c);
+      const Candidate q = candidate(order_of(to_float(x[c])), c);
       if (q < last && q > mine) mine = q;
     }
     for (int d = 16; d > 0; d >>= 1) {
-      const unsigned long long o = __shfl_xor_sync(0xffffffffu, mine, d);
+      const Candidate o = __shfl_xor_sync(0xffffffffu, mine, d);
       if (o > mine) mine = o;
     }
     if (lane == 0) best[warp] = mine;
@@ -115,13 +403,13 @@ template <typename T> __global__ void __launch_bounds__(256) log_probs_rows_kern
       if (best[w] > last) last = best[w];
     __syncthreads();
     if (threadIdx.x == 0) {
-      const int c = candidate_index(last);
-      a.top_index[row * a.k + i] = c;
-      a.top[row * a.k + i] = lse == -INFINITY ? -INFINITY : to_float(x[c]) - lse;
+      a.top_index[row * a.k + i] = candidate_index(last);
+      a.top[row * a.k + i] = st.log_prob(value_of((unsigned)(last >> 32)));
     }
   }
 }
 
+// ---- planes ----------------------------------------------------------------------------------------------------------
 template <typename T> __global__ void __launch_bounds__(256) log_probs_planes_kernel(LogProbArgs a) {
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= a.outer * a.inner) return;
@@ -129,62 +417,66 @@ template <typename T> __global__ void __launch_bounds__(256) log_probs_planes_ke
   const T *x = (const T *)a.x + o * a.C * a.inner + i;
   Stats st;
   for (int c = 0; c < a.C; c++) st.add(to_float(x[c * a.inner]));
-  const float lse = st.lse();
   const int64_t t = a.target[at];
-  a.log_probs[at] = target_log_prob(a, t, lse, t >= 0 && t < a.C ? to_float(x[t * a.inner]) : 0.f);
-  a.entropy[at] = st.entropy();
-  if (a.lse) a.lse[at] = lse;
-  unsigned long long last = ~0ull;
+  write_stats(a, at, st, t, t >= 0 && t < a.C ? to_float(x[t * a.inner]) : 0.f);
+  Candidate last = ~0ull;
   for (int j = 0; j < a.k; j++) {
-    unsigned long long mine = 0;
+    Candidate mine = 0;
     for (int c = 0; c < a.C; c++) {
-      const unsigned long long q = candidate(to_float(x[c * a.inner]), c);
+      const Candidate q = candidate(order_of(to_float(x[c * a.inner])), c);
       if (q < last && q > mine) mine = q;
     }
     last = mine;
-    const int c = candidate_index(mine);
     const int64_t to = (o * a.k + j) * a.inner + i;
-    a.top_index[to] = c;
-    a.top[to] = lse == -INFINITY ? -INFINITY : to_float(x[(int64_t)c * a.inner]) - lse;
+    a.top_index[to] = candidate_index(mine);
+    a.top[to] = st.log_prob(value_of((unsigned)(mine >> 32)));
   }
 }
 
+// ---- gradient --------------------------------------------------------------------------------------------------------
 struct LogProbGradArgs {
   const void *x;
   const int64_t *target, *top_index;
-  const float *lse, *entropy, *g, *h, *t;
+  const float2 *stats;
+  const float *entropy, *g, *h, *t;
   void *gx;
   int64_t outer, inner, x_stride, ignore_index, g_stride, h_stride;  // g_stride, h_stride: 1, or 0 for one value for all
   int C, k;
 };
 
-// What the elements of one distribution share.
+// What the elements of one distribution share.  With e = 2^d, d = (x - m) log2 e, p = e / S and log p = ln2 d - ln S:
+//     -p (g + sum t + h (log p + H)) = e (flat + slope d)
 struct RowGrad {
-  float lse, entropy, g, h, all;  // all = g + sum t
+  float m, flat, slope, g;
   int64_t target;
+  bool tops;
   __device__ __forceinline__ float of(float x) const {
-    const float d = x - lse, p = lse == -INFINITY ? 0.f : expf(d);
-    return -p * (all + h * (fmaxf(d, -1e4f) + entropy));
+    const float d = distance(x, m);
+    return exp2_fast(d) * fmaf(slope, d, flat);
   }
 };
 // `at`: the distribution's number, `o`, `i`: its parts.
 __device__ __forceinline__ RowGrad row_grad(const LogProbGradArgs &a, int64_t at, int64_t o, int64_t i) {
   RowGrad r;
-  r.lse = a.lse[at];
-  r.entropy = a.entropy[at];
+  const float2 st = a.stats[at];
+  const bool empty = st.y == 0.f;
+  r.m = st.x;
   r.target = a.target[at];
-  const bool none = r.target == a.ignore_index || !a.g || r.lse == -INFINITY;
-  r.g = none ? 0.f : r.target < 0 || r.target >= a.C ? NAN : a.g[at * a.g_stride];
-  r.h = a.h ? a.h[at * a.h_stride] : 0.f;
-  r.all = r.g;
-  if (a.t && r.lse != -INFINITY)
-    for (int j = 0; j < a.k; j++) r.all += a.t[(o * a.k + j) * a.inner + i];
+  r.tops = a.t != nullptr && !empty;
+  r.g = !a.g || empty || r.target == a.ignore_index ? 0.f : r.target < 0 || r.target >= a.C ? NAN : a.g[at * a.g_stride];
+  const float h = a.h && !empty ? a.h[at * a.h_stride] : 0.f;
+  float all = r.g;
+  if (r.tops)
+    for (int j = 0; j < a.k; j++) all += a.t[(o * a.k + j) * a.inner + i];
+  const float inverse = empty ? 0.f : 1.f / st.y;
+  r.slope = -h * kLn2 * inverse;
+  r.flat = empty ? 0.f : -(all + h * (a.entropy[at] - logf(st.y))) * inverse;
   return r;
 }
 // The class c's own gradients: the target's, and those of the most probable classes.
 __device__ __forceinline__ float own_grad(const LogProbGradArgs &a, const RowGrad &r, int64_t o, int64_t i, int c) {
   float v = c == r.target ? r.g : 0.f;
-  if (a.t && r.lse != -INFINITY)
+  if (r.tops)
     for (int j = 0; j < a.k; j++) {
       const int64_t at = (o * a.k + j) * a.inner + i;
       if (a.top_index[at] == c) v += a.t[at];
@@ -192,12 +484,50 @@ __device__ __forceinline__ float own_grad(const LogProbGradArgs &a, const RowGra
   return v;
 }
 
+// A block takes a run of a row's vectors; the most probable classes are put right behind it.
 template <typename T> __global__ void __launch_bounds__(256) log_probs_rows_grad_kernel(LogProbGradArgs a) {
-  const int64_t row = blockIdx.x;
+  constexpr int N = RowVector<T>::N;
+  const int64_t row = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
+  if (row >= a.outer) return;
   const T *x = (const T *)a.x + row * a.x_stride;
   T *gx = (T *)a.gx + row * a.C;
   const RowGrad r = row_grad(a, row, row, 0);
-  for (int c = threadIdx.x; c < a.C; c += 256) gx[c] = from_float<T>(r.of(to_float(x[c])) + own_grad(a, r, row, 0, c));
+  const int shift = RowVector<T>::shift_of(gx), vectors = (int)(((int64_t)a.C + shift + N - 1) / N);
+  const bool alike = RowVector<T>::shift_of(x) == shift;
+  const int per = (vectors + (int)gridDim.x - 1) / (int)gridDim.x, from = min((int)blockIdx.x * per, vectors), end = min(from + per, vectors);
+  const T none = from_float<T>(-INFINITY);
+  const int target = r.target >= 0 && r.target < a.C ? (int)r.target : -1;
+  for (int v0 = from; v0 < end; v0 += 256 * 4) {
+    RowVector<T> v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int at = v0 + i * 256 + threadIdx.x, first = at < end ? at * N - shift : a.C;
+      if (alike) {
+        v[i].load(x, first, a.C, none);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; j++) v[i].t[j] = first + j >= 0 && first + j < a.C ? x[first + j] : none;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int at = v0 + i * 256 + threadIdx.x, first = at < end ? at * N - shift : a.C;
+#pragma unroll
+      for (int j = 0; j < N; j++) {
+        const float d = r.of(v[i].at(j));
+        v[i].t[j] = from_float<T>(first + j == target ? d + r.g : d);
+      }
+      v[i].store(gx, first, a.C);
+    }
+  }
+  if (!r.tops) return;
+  __syncthreads();
+  for (int j = threadIdx.x; j < a.k; j += 256) {
+    const int64_t c = a.top_index[row * a.k + j];
+    if (c < 0 || c >= a.C) continue;
+    const int v = (int)((c + shift) / N);
+    if (v >= from && v < end) gx[c] = from_float<T>(r.of(to_float(x[c])) + own_grad(a, r, row, 0, (int)c));
+  }
 }
 
 template <typename T> __global__ void __launch_bounds__(256) log_probs_planes_grad_kernel(LogProbGradArgs a) {
@@ -207,6 +537,39 @@ template <typename T> __global__ void __launch_bounds__(256) log_probs_planes_gr
   const RowGrad r = row_grad(a, at, o, i);
   for (int c = 0; c < a.C; c++)
     ((T *)a.gx)[base + c * a.inner] = from_float<T>(r.of(to_float(((const T *)a.x)[base + c * a.inner])) + own_grad(a, r, o, i, c));
+}
+
+// Blocks for a row: enough for two on each SM, no more than the row has tiles.
+inline int blocks_per_row(int64_t rows, int64_t C, int64_t tile, int most) {
+  const int64_t tiles = (C + tile - 1) / tile;
+  int n = 1;
+  while (n < most && n < tiles && n * rows < 2 * 148) n *= 2;
+  return n;
+}
+// Rows as a grid's second and third dimension.
+inline dim3 row_grid(int n, int64_t rows) {
+  const unsigned y = rows < 32768 ? (unsigned)rows : 32768u;
+  return dim3((unsigned)n, y, (unsigned)((rows + y - 1) / y));
+}
+
+template <typename T> cudaError_t launch_rows(const LogProbArgs &a, cudaStream_t st) {
+  const int n = blocks_per_row(a.outer, a.C, kRowTile, kMostCluster);
+  void (*kernel)(LogProbArgs) = a.k > 0 ? log_probs_rows_kernel<T, true> : log_probs_rows_kernel<T, false>;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = row_grid(n, a.outer);
+  config.blockDim = dim3(kRowThreads);
+  config.stream = st;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = (unsigned)n;
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  if (n > 8) {
+    const cudaError_t e = cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaLaunchKernelEx(&config, kernel, a);
 }
 
 inline int log_probs_sizes(int64_t outer, int64_t C, int64_t inner, int64_t k) {
@@ -220,7 +583,7 @@ inline int log_probs_sizes(int64_t outer, int64_t C, int64_t inner, int64_t k) {
 
 using namespace sph;
 
-extern "C" int sph_token_log_probs_forward(const void *x, const int64_t *target, float *log_probs, float *entropy, float *lse,
+extern "C" int sph_token_log_probs_forward(const void *x, const int64_t *target, float *log_probs, float *entropy, float *stats,
                                            float *top, int64_t *top_index, int64_t outer, int64_t C, int64_t inner, int64_t x_stride,
                                            int64_t k, int64_t ignore_index, int dtype, void *stream) {
   SPH_RANGE("sph_token_log_probs_forward");
@@ -229,18 +592,25 @@ extern "C" int sph_token_log_probs_forward(const void *x, const int64_t *target,
   if (outer == 0) return SPH_OK;
   if (!x || !target || !log_probs || !entropy || (k > 0 && (!top || !top_index)) || (inner == 1 && outer > 1 && x_stride < C))
     return SPH_ERR_INVALID_ARGUMENT;
-  const LogProbArgs a{x, target, log_probs, entropy, lse, top, top_index, outer, inner, x_stride, ignore_index, (int)C, (int)k};
+  const LogProbArgs a{x, target, log_probs, entropy, top, (float2 *)stats, top_index, outer, inner, x_stride, ignore_index, (int)C, (int)k};
   cudaStream_t st = (cudaStream_t)stream;
   SPH_DISPATCH_ELEMENT(dtype, {
-    if (inner == 1)
-      log_probs_rows_kernel<T><<<(unsigned)outer, 256, 0, st>>>(a);
-    else
+    if (inner == 1 && C <= 1024 - RowVector<T>::N)  // (a row's start may take a part of a vector)
+      (k > 0 ? log_probs_warp_kernel<T, true> : log_probs_warp_kernel<T, false>)<<<(unsigned)((outer + 7) / 8), 256, 0, st>>>(a);
+    else if (inner == 1 && k > kMostTop)
+      log_probs_many_kernel<T><<<(unsigned)outer, 256, 0, st>>>(a);
+    else if (inner == 1) {
+      if (launch_rows<T>(a, st) != cudaSuccess) {
+        cudaGetLastError();
+        return SPH_ERR_CUDA;
+      }
+    } else
       log_probs_planes_kernel<T><<<(unsigned)((outer * inner + 255) / 256), 256, 0, st>>>(a);
   });
   return launch_status();
 }
 
-extern "C" int sph_token_log_probs_backward(const void *x, const int64_t *target, const float *lse, const float *entropy,
+extern "C" int sph_token_log_probs_backward(const void *x, const int64_t *target, const float *stats, const float *entropy,
                                             const int64_t *top_index, const float *g, int64_t g_stride, const float *h,
                                             int64_t h_stride, const float *t, void *gx, int64_t outer, int64_t C, int64_t inner,
                                             int64_t x_stride, int64_t k, int64_t ignore_index, int dtype, void *stream) {
@@ -248,15 +618,15 @@ extern "C" int sph_token_log_probs_backward(const void *x, const int64_t *target
   if (!element_dtype(dtype)) return SPH_ERR_UNSUPPORTED;
   if (const int rc = log_probs_sizes(outer, C, inner, k)) return rc;
   if (outer == 0) return SPH_OK;
-  if (!x || !target || !lse || !entropy || !gx || (t && (k == 0 || !top_index)) || (inner == 1 && outer > 1 && x_stride < C) ||
+  if (!x || !target || !stats || !entropy || !gx || (t && (k == 0 || !top_index)) || (inner == 1 && outer > 1 && x_stride < C) ||
       g_stride < 0 || g_stride > 1 || h_stride < 0 || h_stride > 1)
     return SPH_ERR_INVALID_ARGUMENT;
-  const LogProbGradArgs a{x, target, top_index, lse, entropy, g, h, t, gx, outer, inner, x_stride, ignore_index, g_stride, h_stride,
+  const LogProbGradArgs a{x, target, top_index, (const float2 *)stats, entropy, g, h, t, gx, outer, inner, x_stride, ignore_index, g_stride, h_stride,
                           (int)C, (int)k};
   cudaStream_t st = (cudaStream_t)stream;
   SPH_DISPATCH_ELEMENT(dtype, {
     if (inner == 1)
-      log_probs_rows_grad_kernel<T><<<(unsigned)outer, 256, 0, st>>>(a);
+      log_probs_rows_grad_kernel<T><<<row_grid(blocks_per_row(outer, C, 256 * RowVector<T>::N, 64), outer), 256, 0, st>>>(a);
     else
       log_probs_planes_grad_kernel<T><<<(unsigned)((outer * inner + 255) / 256), 256, 0, st>>>(a);
   });

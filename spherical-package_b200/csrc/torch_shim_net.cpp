@@ -260,14 +260,14 @@ std::vector<Tensor> rms_norm_quantized(const Tensor &x, const OptTensor &weight,
 
 // ---- log probabilities -----------------------------------------------------------------------------------------------
 struct LogProbsNode : public Node {
-  SavedVariable x, target, lse, entropy, top_index;
+  SavedVariable x, target, stats, entropy, top_index;
   Layout layout;
   int64_t k = 0, ignore_index = 0;
   std::mutex mu;
   std::string name() const override { return "TokenLogProbsBackward"; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mu);
-    for (SavedVariable *v : {&x, &target, &lse, &entropy, &top_index}) v->reset_data();
+    for (SavedVariable *v : {&x, &target, &stats, &entropy, &top_index}) v->reset_data();
   }
   // One value for all (the gradient of a sum or a mean) is taken as such.
   static const float *spread(Tensor &g, int64_t &stride) {
@@ -286,7 +286,7 @@ struct LogProbsNode : public Node {
     variable_list r(1);
     {
       at::NoGradGuard no_grad;
-      const Tensor in = x.unpack(), t = target.unpack(), s = lse.unpack(), e = entropy.unpack(shared_from_this()), index = top_index.unpack();
+      const Tensor in = x.unpack(), t = target.unpack(), s = stats.unpack(), e = entropy.unpack(shared_from_this()), index = top_index.unpack();
       if (!task_should_compute_output(0)) return r;
       const Layout &l = layout;
       c10::cuda::CUDAGuard guard(in.device());
@@ -319,7 +319,7 @@ c10::optional<std::vector<Tensor>> token_log_probs(const Tensor &x, const Tensor
   check_device(target, "target", x);
   const bool train = wants_grad({&x});
   std::vector<Tensor> out;
-  Tensor lse, index;
+  Tensor stats, index;
   {
     at::NoGradGuard no_grad;
     c10::cuda::CUDAGuard guard(x.device());
@@ -329,9 +329,9 @@ c10::optional<std::vector<Tensor>> token_log_probs(const Tensor &x, const Tensor
       out.push_back(like_layout(x, l, k, torch::kFloat));
       index = like_layout(x, l, k, torch::kLong);
     }
-    if (train) lse = torch::empty(target.sizes(), f32);
+    if (train) stats = torch::empty({target.numel(), 2}, f32);
     ok(sph_token_log_probs_forward(x.data_ptr(), target.data_ptr<int64_t>(), out[0].data_ptr<float>(), out[1].data_ptr<float>(),
-                                   train ? lse.data_ptr<float>() : nullptr, k > 0 ? out[2].data_ptr<float>() : nullptr,
+                                   train ? stats.data_ptr<float>() : nullptr, k > 0 ? out[2].data_ptr<float>() : nullptr,
                                    k > 0 ? index.data_ptr<int64_t>() : nullptr, l.outer, l.C, l.inner, l.stride, k, ignore_index, dtype,
                                    current_stream()),
        "sph_token_log_probs_forward");
@@ -344,7 +344,7 @@ c10::optional<std::vector<Tensor>> token_log_probs(const Tensor &x, const Tensor
     torch::autograd::set_history(out, n);
     n->x = SavedVariable(x, false);
     n->target = SavedVariable(target, false);
-    n->lse = SavedVariable(lse, false);
+    n->stats = SavedVariable(stats, false);
     n->entropy = SavedVariable(out[1], true);
     n->top_index = SavedVariable(index, false);
   }
