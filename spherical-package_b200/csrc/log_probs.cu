@@ -115,37 +115,6 @@ __device__ __forceinline__ void write_stats(const LogProbArgs &a, int64_t at, co
 }
 
 // ---- rows ------------------------------------------------------------------------------------------------------------
-// 16 bytes of a row at a time.  A row need not start on a 16-byte boundary: vector v holds the elements [v n - shift, v n - shift + n)
-// with `shift` the elements between the boundary before the row and its start; the vectors at its two ends are put together
-// from single elements.
-template <typename T> struct RowVector {
-  static constexpr int N = 16 / (int)sizeof(T);
-  union {
-    uint4 u;
-    T t[N];
-  };
-  static __device__ __forceinline__ int shift_of(const T *row) { return (int)((uintptr_t)row % 16 / sizeof(T)); }
-  // Elements outside the row are `outside`.
-  __device__ __forceinline__ void load(const T *row, int first, int C, T outside) {
-    if (first >= 0 && first + N <= C) {
-      u = *(const uint4 *)(row + first);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; i++) t[i] = first + i >= 0 && first + i < C ? row[first + i] : outside;
-    }
-  }
-  __device__ __forceinline__ void store(T *row, int first, int C) const {
-    if (first >= 0 && first + N <= C) {
-      *(uint4 *)(row + first) = u;
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; i++)
-        if (first + i >= 0 && first + i < C) row[first + i] = t[i];
-    }
-  }
-  __device__ __forceinline__ float at(int i) const { return to_float(t[i]); }
-};
-
 // A thread's part of a tile: 32 logits in registers.
 template <typename T> struct Tile {
   static constexpr int N = RowVector<T>::N, V = 32 / N;
