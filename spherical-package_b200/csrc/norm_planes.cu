@@ -1,0 +1,114 @@
+// Norms over the channels of planes, forward; see norm.cuh for the formulas, planes.cuh for how the planes are read.
+#include "norm.cuh"
+#include "planes.cuh"
+
+namespace sph {
+
+template <typename T, bool E4M3, bool ADD, int MODE, int LOG> __global__ void __launch_bounds__(kPlaneThreads, 4) norm_planes_kernel(NormArgs a, PlaneTile tile) {
+  using L = Lane<T, MODE, LOG>;
+  using G = Geometry<T, MODE, LOG>;
+  constexpr int N = L::N;
+  __shared__ float shared[2][kPlaneThreads * N];
+  __shared__ float weight[kMostPlanes];
+  constexpr int ACROSS = G::ACROSS;
+  const int first = (threadIdx.x >> 5) & (ACROSS - 1);
+  const Run<MODE, G::PIXELS> run(tile, blockIdx.x, a.outer, a.C, a.inner);
+  T *s = (T *)plane_memory, *add = s + a.C * G::PITCH;
+  copy_run<T, MODE, LOG>(s, (const T *)a.x, run);
+  if (ADD) copy_run<T, MODE, LOG>(add, (const T *)a.residual, run);
+  copies_end();
+  keep_weights<T>(weight, a.weight, a.weight_f32, a.C);
+  const L px(run, first);
+  const int64_t step = ACROSS * a.inner;
+  const int shift = MODE == kShifted ? shift_of((const T *)a.x + run.offset(0), 0, first, a.inner) : 0;
+  T *mine = s + first * G::PITCH + px.col + shift;
+  const T *other = ADD ? add + first * G::PITCH + px.col + (MODE == kShifted ? shift_of((const T *)a.residual + run.offset(0), 0, first, a.inner) : 0) : nullptr;
+  copies_wait<0>();
+  __syncthreads();
+  float v[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) v[i] = 0.f;
+  {
+    T *p = mine;
+    int64_t plane = 0;
+#pragma unroll 8
+    for (int c = first; c < a.C; c += ACROSS, p += G::ROW, plane += step) {
+      Pixels<T> q = L::load(p);
+      if (ADD) {
+        const Pixels<T> o = L::load(other + (p - mine));
+#pragma unroll
+        for (int i = 0; i < N; i++) q.t[i] = from_float<T>(to_float(q.t[i]) + to_float(o.t[i]));
+        L::keep(p, q);
+        px.store((T *)a.sum, plane, q);
+      }
+#pragma unroll
+      for (int i = 0; i < N; i++) v[i] = fmaf(to_float(q.t[i]), to_float(q.t[i]), v[i]);
+    }
+  }
+  plane_join<LOG>(v, shared[0], [](float p, float q) { return p + q; });
+  float rstd[N], scale[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    rstd[i] = 1.f / sqrtf(v[i] * a.inv_c + a.eps);
+    if (first == 0 && px.in[i] && a.rstd) a.rstd[px.norm[i]] = rstd[i];
+    scale[i] = 1.f;
+  }
+  if (E4M3) {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = 0.f;
+    const T *p = mine;
+#pragma unroll 8
+    for (int c = first; c < a.C; c += ACROSS, p += G::ROW) {
+      const Pixels<T> q = L::load(p);
+#pragma unroll
+      for (int i = 0; i < N; i++) v[i] = max_nan(v[i], fabsf(to_float(q.t[i]) * rstd[i] * weight[c]));
+    }
+    plane_join<LOG>(v, shared[1], [](float p, float q) { return max_nan(p, q); });
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const Scale sc = Scale::of(v[i]);
+      scale[i] = sc.inverse;
+      if (first == 0 && px.in[i]) a.scale[px.norm[i]] = sc.scale;
+    }
+  }
+  const T *p = mine;
+  int64_t plane = 0;
+#pragma unroll 8
+  for (int c = first; c < a.C; c += ACROSS, p += G::ROW, plane += step) {
+    Pixels<T> q = L::load(p);
+    float y[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) y[i] = to_float(q.t[i]) * rstd[i] * weight[c];
+    if (E4M3) {
+#pragma unroll
+      for (int i = 0; i < N; i++) y[i] *= scale[i];
+      px.store_e4m3((__nv_fp8_storage_t *)a.out, plane, y);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i++) q.t[i] = from_float<T>(y[i]);
+      px.store((T *)a.out, plane, q);
+    }
+  }
+}
+
+template <typename T, bool E4M3> void norm_planes_launch(const NormArgs &a, cudaStream_t st) {
+  const Mode mode = plane_mode<T>(a.C, a.inner, planes_aligned<T>(a.inner, {a.x, a.residual, a.sum, a.out}));
+  SPH_DISPATCH_PLANES(mode, a.C, {
+    const PlaneTile tile = PlaneTile::of<G, MODE>(a.outer, a.inner);
+    if (a.residual)
+      plane_launch<G, T>(norm_planes_kernel<T, E4M3, true, MODE, LOG>, a, tile, 2, (unsigned)tile.runs, st);
+    else
+      plane_launch<G, T>(norm_planes_kernel<T, E4M3, false, MODE, LOG>, a, tile, 1, (unsigned)tile.runs, st);
+  })
+}
+
+void norm_planes_forward(const NormArgs &a, int dtype, cudaStream_t st) {
+  SPH_DISPATCH_ELEMENT(dtype, {
+    if (a.scale)
+      norm_planes_launch<T, true>(a, st);
+    else
+      norm_planes_launch<T, false>(a, st);
+  });
+}
+
+}  // namespace sph

@@ -1,0 +1,255 @@
+// Runs of pixels with all their channels in shared memory.
+#pragma once
+
+#include <algorithm>
+#include <initializer_list>
+
+#include "element.cuh"
+
+namespace sph {
+
+// ---- planes through shared memory ------------------------------------------------------------------------------------
+// A block of 8 warps takes a run of pixels with all their channels into shared memory by asynchronous copies, so that every
+// tensor is read and written once; two or more blocks a SM copy and compute in turn.  `across` warps share the channels of a
+// unit of 32 float32 or 64 16-bit pixels, the others have further units; what a norm needs of all its channels is joined
+// through shared memory.  Rows of a channel are copied
+//   kWide    16 bytes at a time, where planes start on 16-byte boundaries; a lane has 4 bytes, neighbouring pixels;
+//   kShifted 16 bytes at a time too, from the boundary before the run on, so that a row lies in shared memory as far off a
+//            boundary as in its tensor; a lane has every 32nd pixel, and a run stays in its image;
+//   kSingle  pixel by pixel (small images, few channels).
+enum Mode { kWide, kShifted, kSingle };
+template <typename T> union Pixels {  // a lane's, of a channel
+  static constexpr int N = 4 / (int)sizeof(T), V = 16 / (int)sizeof(T);
+  unsigned w;
+  T t[N];
+  __device__ __forceinline__ Pixels() {}
+};
+constexpr int kPlaneWarps = 8, kPlaneThreads = 32 * kPlaneWarps, kMostPlanes = 512;
+// LOG: log2 of the warps that share a unit's channels, 0 (one warp has them all) or 3.
+template <typename T, int MODE, int LOG> struct Geometry {
+  static constexpr int N = Pixels<T>::N, V = Pixels<T>::V;
+  static constexpr int ACROSS = 1 << LOG, PIXELS = 256 * N >> LOG;  // of a run
+  static constexpr int PITCH = PIXELS + (MODE == kShifted ? V : 0);  // elements from a channel's row to the next
+  static constexpr int ROW = ACROSS * PITCH;                         // to a warp's next channel
+};
+struct PlaneTile {
+  FastDiv by;    // by the pixels of a plane, or, shifted, by a plane's runs
+  bool small;    // fewer than 2^31 pixels in all
+  int64_t runs;  // in all
+  template <class G, int MODE> static PlaneTile of(int64_t outer, int64_t inner) {
+    PlaneTile t;
+    const int64_t total = outer * inner, each = (inner + G::PIXELS - 1) / G::PIXELS;
+    t.runs = MODE == kShifted ? outer * each : (total + G::PIXELS - 1) / G::PIXELS;
+    t.small = total < ((int64_t)1 << 31);
+    t.by = FastDiv::make(!t.small ? 1u : (unsigned)(MODE == kShifted ? each : inner));
+    return t;
+  }
+};
+// Channels one warp may have alone; with more, eight share them.
+constexpr int kAlone = 32;
+// Runs that end with their image are to be an eighth more at most.
+template <typename T> Mode plane_mode(int64_t C, int64_t inner, bool aligned) {
+  using G = Geometry<T, kShifted, 3>;
+  return aligned ? kWide : C > kAlone && 8 * ((inner + G::PIXELS - 1) / G::PIXELS * G::PIXELS) <= 9 * inner ? kShifted : kSingle;
+}
+
+// A run of pixels: offset of channel 0 of its pixel i, and the norms' numbers.
+template <int MODE, int PIXELS> struct Run {
+  int64_t start, image, inner, total;  // kShifted: start and image are this run's, else pixels are numbered through
+  int C;
+  const PlaneTile &tile;
+  __device__ __forceinline__ Run(const PlaneTile &tile, int64_t index, int64_t outer, int C, int64_t inner)
+      : inner(inner), total(outer * inner), C(C), tile(tile) {
+    if (MODE == kShifted) {
+      const int64_t each = (inner + PIXELS - 1) / PIXELS;
+      image = tile.small ? (int64_t)tile.by.div((unsigned)index) : index / each;
+      start = (index - image * each) * PIXELS;
+    } else {
+      start = index * PIXELS;
+    }
+  }
+  __device__ __forceinline__ bool has(int i) const { return MODE == kShifted ? start + i < inner : start + i < total; }
+  __device__ __forceinline__ int64_t norm(int i) const { return MODE == kShifted ? image * inner + start + i : start + i; }
+  __device__ __forceinline__ int64_t offset(int i) const {
+    if (MODE == kShifted) return image * C * inner + start + i;
+    const int64_t at = start + i, o = tile.small ? (int64_t)tile.by.div((unsigned)at) : at / inner;
+    return o * C * inner + (at - o * inner);
+  }
+};
+
+__device__ __forceinline__ void copy_16(void *to, const void *from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_4(void *to, const void *from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
+
+// Elements between the 16-byte boundary before a channel's run and the run (kShifted), the same for a warp's channels.
+template <typename T> __device__ __forceinline__ int shift_of(const T *from, int64_t offset, int c, int64_t inner) {
+  return (int)(((uintptr_t)(from + offset) / sizeof(T) + (uintptr_t)c * (uintptr_t)inner) & (Pixels<T>::V - 1));
+}
+
+// Copies a run, all channels.
+template <typename T, int MODE, int LOG, class R> __device__ __forceinline__ void copy_run(T *to, const T *from, const R &run) {
+  using G = Geometry<T, MODE, LOG>;
+  constexpr int V = G::V;
+  if constexpr (MODE == kWide) {
+    constexpr int COLS = G::PIXELS / V, ROWS = kPlaneThreads / COLS;
+    const int col = (threadIdx.x % COLS) * V, first = threadIdx.x / COLS;
+    if (!run.has(col)) return;
+    const T *p = from + run.offset(col) + first * run.inner;
+    const int64_t step = ROWS * run.inner;
+    T *q = to + first * G::PITCH + col;
+#pragma unroll 4
+    for (int c = first; c < run.C; c += ROWS, p += step, q += ROWS * G::PITCH) copy_16(q, p);
+  } else if constexpr (MODE == kShifted) {
+    constexpr int PIECES = G::PIXELS / V + 1;  // a row's, from the boundary before it
+    const T *base = from + run.offset(0), *last = from + run.total * run.C;
+    const int count = (int)min((int64_t)G::PIXELS, run.inner - run.start);
+#pragma unroll 4
+    for (int i = threadIdx.x; i < run.C * PIECES; i += kPlaneThreads) {
+      const int c = i / PIECES, j = i % PIECES, at = j * V - shift_of(base, 0, c, run.inner);
+      if (at >= count) continue;
+      const T *p = base + c * run.inner + at;
+      T *q = to + c * G::PITCH + j * V;
+      if (p >= from && p + V <= last) {
+        copy_16(q, p);
+      } else {  // the tensor's first and last pixels
+        for (int e = 0; e < V; e++)
+          if (at + e >= 0 && at + e < count) q[e] = p[e];
+      }
+    }
+  } else {
+    constexpr int COLS = G::PIXELS < kPlaneThreads ? G::PIXELS : kPlaneThreads, ROWS = kPlaneThreads / COLS;
+#pragma unroll
+    for (int col = threadIdx.x % COLS; col < G::PIXELS; col += COLS) {
+      if (!run.has(col)) return;
+      const int first = threadIdx.x / COLS;
+      const T *p = from + run.offset(col) + first * run.inner;
+      const int64_t step = ROWS * run.inner;
+      T *q = to + first * G::PITCH + col;
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll 4
+        for (int c = first; c < run.C; c += ROWS, p += step, q += ROWS * G::PITCH) copy_4(q, p);
+      } else {
+        for (int c = first; c < run.C; c += ROWS * 16) {
+          T v[16];
+#pragma unroll
+          for (int e = 0; e < 16; e++)
+            if (c + e * ROWS < run.C) v[e] = p[e * step];
+#pragma unroll
+          for (int e = 0; e < 16; e++)
+            if (c + e * ROWS < run.C) q[e * ROWS * G::PITCH] = v[e];
+          p += 16 * step, q += 16 * ROWS * G::PITCH;
+        }
+      }
+    }
+  }
+}
+
+// A lane's pixels of a run: col, col + 1 (kWide) or col, col + 32.
+template <typename T, int MODE, int LOG> struct Lane {
+  static constexpr int N = Pixels<T>::N, STEP = MODE == kWide ? 1 : 32;
+  int col;
+  bool in[N];
+  int64_t norm[N], off[N];  // of the warp's first channel
+  template <class R> __device__ __forceinline__ Lane(const R &run, int first) {
+    const int lane = threadIdx.x & 31;
+    col = (threadIdx.x >> 5 >> LOG) * 32 * N + (MODE == kWide ? lane * N : lane);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      in[i] = run.has(col + i * STEP);
+      norm[i] = run.norm(col + i * STEP);
+      off[i] = in[i] && (MODE != kWide || i == 0) ? run.offset(col + i * STEP) + first * run.inner : 0;
+    }
+  }
+  static __device__ __forceinline__ Pixels<T> load(const T *p) {
+    Pixels<T> v;
+    if (MODE == kWide) v.w = *(const unsigned *)p;
+    else {
+#pragma unroll
+      for (int i = 0; i < N; i++) v.t[i] = p[i * STEP];
+    }
+    return v;
+  }
+  static __device__ __forceinline__ void keep(T *p, const Pixels<T> &v) {
+    if (MODE == kWide) *(unsigned *)p = v.w;
+    else {
+#pragma unroll
+      for (int i = 0; i < N; i++) p[i * STEP] = v.t[i];
+    }
+  }
+  // `plane`: elements from the warp's first channel.
+  __device__ __forceinline__ void store(T *to, int64_t plane, const Pixels<T> &v) const {
+    if (MODE == kWide) {
+      if (in[0]) *(unsigned *)(to + off[0] + plane) = v.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i++)
+        if (in[i]) to[off[i] + plane] = v.t[i];
+    }
+  }
+  __device__ __forceinline__ void store_e4m3(__nv_fp8_storage_t *to, int64_t plane, const float (&y)[N]) const {
+    if (MODE == kWide && N == 2) {
+      if (in[0]) *(__nv_fp8x2_storage_t *)(to + off[0] + plane) = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[N - 1]), __NV_SATFINITE, __NV_E4M3);
+    } else if (MODE == kWide) {
+      if (in[0]) to[off[0] + plane] = to_e4m3(y[0]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i++)
+        if (in[i]) to[off[i] + plane] = to_e4m3(y[i]);
+    }
+  }
+};
+
+// Joins a value of each of the lane's pixels over the warps that share them.  `shared`: 8 x 32 x N floats.
+template <int LOG, int N, class F> __device__ __forceinline__ void plane_join(float (&v)[N], float *shared, F f) {
+  if (LOG == 0) return;
+  constexpr int n = 1 << LOG;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mates = warp & ~(n - 1);
+#pragma unroll
+  for (int i = 0; i < N; i++) shared[(warp * N + i) * 32 + lane] = v[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; i++) v[i] = shared[(mates * N + i) * 32 + lane];
+#pragma unroll
+  for (int w = 1; w < n; w++)
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = f(v[i], shared[((mates + w) * N + i) * 32 + lane]);
+}
+
+// The weights as floats, ones without.
+template <typename T> __device__ __forceinline__ void keep_weights(float *to, const void *w, bool f32, int C) {
+  for (int c = threadIdx.x; c < C; c += kPlaneThreads) to[c] = w ? load_weight<T>(w, c, f32) : 1.f;
+}
+
+extern __shared__ __align__(16) unsigned char plane_memory[];
+
+// Whether 16 bytes of a plane may be copied at once.
+template <typename T> bool planes_aligned(int64_t inner, std::initializer_list<const void *> ps) {
+  uintptr_t bits = (uintptr_t)inner * sizeof(T);
+  for (const void *p : ps) bits |= (uintptr_t)p;
+  return bits % 16 == 0;
+}
+// Launches a kernel over runs of `tensors` tensors in shared memory.
+template <class G, typename T, class A>
+void plane_launch(void (*kernel)(A, PlaneTile), const A &a, const PlaneTile &tile, int tensors, unsigned blocks, cudaStream_t st) {
+  const int bytes = (int)sizeof(T) * a.C * G::PITCH * tensors;
+  if (bytes > 32768) cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  kernel<<<blocks, kPlaneThreads, bytes, st>>>(a, tile);
+}
+// Run a statement with MODE, LOG and the geometry G.
+#define SPH_PLANES(M, L, ...) { constexpr int MODE = M, LOG = L; using G = Geometry<T, MODE, LOG>; __VA_ARGS__; }
+#define SPH_DISPATCH_PLANES(mode, C, ...)                              \
+  if (C <= kAlone) {                                                   \
+    if (mode == kWide) SPH_PLANES(kWide, 0, __VA_ARGS__)               \
+    else SPH_PLANES(kSingle, 0, __VA_ARGS__)                           \
+  } else {                                                             \
+    if (mode == kWide) SPH_PLANES(kWide, 3, __VA_ARGS__)               \
+    else if (mode == kShifted) SPH_PLANES(kShifted, 3, __VA_ARGS__)    \
+    else SPH_PLANES(kSingle, 3, __VA_ARGS__)                           \
+  }
+
+}  // namespace sph
