@@ -47,8 +47,12 @@ __device__ __forceinline__ float from_e4m3(__nv_fp8_storage_t v) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3)));
 }
 
-// Largest magnitude so far; NaN stays.
-__device__ __forceinline__ float max_nan(float a, float b) { return b > a || b != b ? b : a; }
+// max that keeps NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
 // Sums (or other joins) over the threads of a warp or of a block; every thread gets the same value.
 template <class F> __device__ __forceinline__ float warp_join(float v, F f) {
@@ -70,6 +74,16 @@ template <class F> __device__ __forceinline__ float block_join(float v, float *s
   __syncthreads();
   return r;
 }
+
+// Asynchronous copies into shared memory.
+__device__ __forceinline__ void copy_16(void *to, const void *from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_4(void *to, const void *from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
 
 // 16 bytes of a row at a time.  A row need not start on a 16-byte boundary: vector v holds the elements [v n - shift, v n - shift + n)
 // with `shift` the elements between the boundary before the row and its start; the vectors at its two ends are put together

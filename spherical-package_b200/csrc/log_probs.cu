@@ -30,12 +30,6 @@ struct LogProbArgs {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// max that keeps NaN.
-__device__ __forceinline__ float fmax_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 // 2^d for d <= 0 (or NaN), 0 far below.
 __device__ __forceinline__ float exp2_fast(float d) {
   float r;
@@ -44,7 +38,7 @@ __device__ __forceinline__ float exp2_fast(float d) {
 }
 // log2 e times a logit's distance from the maximum; what is infinitely far below stops at a finite distance whose exponential
 // is 0, so that 0 times it is 0.
-__device__ __forceinline__ float distance(float x, float base) { return fmax_nan((x - base) * kLog2e, -1000.f); }
+__device__ __forceinline__ float distance(float x, float base) { return max_nan((x - base) * kLog2e, -1000.f); }
 
 // Order of the candidates as one number: larger is better; value first (NaN above all), then the lower index.
 __device__ __forceinline__ unsigned order_of(float v) {
@@ -80,13 +74,13 @@ struct Stats {
     m = n;
   }
   __device__ __forceinline__ void add(float x) {
-    move_to(fmax_nan(m, x));
+    move_to(max_nan(m, x));
     const float d = distance(x, base(m)), e = exp2_fast(d);
     s += e;
     t = fmaf(e, d, t);
   }
   __device__ __forceinline__ void join(Stats o) {
-    const float n = fmax_nan(m, o.m);
+    const float n = max_nan(m, o.m);
     move_to(n);
     o.move_to(n);
     s += o.s;
@@ -96,7 +90,7 @@ struct Stats {
   __device__ __forceinline__ void join_warp() {
     float n = m;
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) n = fmax_nan(n, __shfl_xor_sync(0xffffffffu, n, d));
+    for (int d = 16; d > 0; d >>= 1) n = max_nan(n, __shfl_xor_sync(0xffffffffu, n, d));
     move_to(n);
     s = warp_sum(s);
     t = warp_sum(t);
@@ -130,11 +124,11 @@ template <typename T> struct Tile {
 #pragma unroll
     for (int i = 0; i < V; i++)
 #pragma unroll
-      for (int j = 0; j < N; j++) m = fmax_nan(m, v[i].at(j));
+      for (int j = 0; j < N; j++) m = max_nan(m, v[i].at(j));
     return m;
   }
   __device__ __forceinline__ void add_to(Stats &st, float largest) const {
-    st.move_to(fmax_nan(st.m, largest));
+    st.move_to(max_nan(st.m, largest));
     const float base = Stats::base(st.m);
     float s[2] = {0.f, 0.f}, t[2] = {0.f, 0.f};
 #pragma unroll

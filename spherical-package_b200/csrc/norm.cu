@@ -250,7 +250,7 @@ template <typename T, bool E4M3, int N, int E, bool WARP> __global__ void __laun
       if (r) add[i].load(r + c);
     }
   }
-  float sq = 0.f;
+  float sq = 0.f, most = 0.f;  // sum of squares; largest |s w|
 #pragma unroll
   for (int i = 0; i < V; i++) {
     const int c = (thread + i * threads) * N;
@@ -260,27 +260,29 @@ template <typename T, bool E4M3, int N, int E, bool WARP> __global__ void __laun
         for (int j = 0; j < N; j++) s[i].t[j] = from_float<T>(to_float(s[i].t[j]) + to_float(add[i].t[j]));
         s[i].store((T *)a.sum + row * a.C + c);
       }
+      float w[N];
+      if (E4M3) load_weights<T, N>(a.weight, c, a.weight_f32, w);
 #pragma unroll
-      for (int j = 0; j < N; j++) sq = fmaf(to_float(s[i].t[j]), to_float(s[i].t[j]), sq);
+      for (int j = 0; j < N; j++) {
+        const float f = to_float(s[i].t[j]);
+        sq = fmaf(f, f, sq);
+        if (E4M3) most = max_nan(most, fabsf(f * w[j]));
+      }
     }
+  }
+  if (E4M3) {  // both joins behind one barrier
+    most = warp_join(most, [](float p, float q) { return max_nan(p, q); });
+    if (!WARP && (threadIdx.x & 31) == 0) shared[1][threadIdx.x >> 5] = most;
   }
   const float rstd = 1.f / sqrtf(row_sum<WARP>(sq, shared[0]) * a.inv_c + a.eps);
   if (thread == 0 && a.rstd) a.rstd[row] = rstd;
-  Scale sc{1.f, 1.f};
+  float factor = rstd;
   if (E4M3) {
-    float amax = 0.f;
-#pragma unroll
-    for (int i = 0; i < V; i++) {
-      const int c = (thread + i * threads) * N;
-      if (c < a.C) {
-        float w[N];
-        load_weights<T, N>(a.weight, c, a.weight_f32, w);
-#pragma unroll
-        for (int j = 0; j < N; j++) amax = max_nan(amax, fabsf(to_float(s[i].t[j]) * rstd * w[j]));
-      }
-    }
-    sc = Scale::of(row_join<WARP>(amax, shared[1], [](float p, float q) { return max_nan(p, q); }, 0.f));
+    const int lane = threadIdx.x & 31;
+    if (!WARP) most = warp_join(lane < (int)(blockDim.x >> 5) ? shared[1][lane] : 0.f, [](float p, float q) { return max_nan(p, q); });
+    const Scale sc = Scale::of(most * rstd);
     if (thread == 0) a.scale[row] = sc.scale;
+    factor *= sc.inverse;
   }
 #pragma unroll
   for (int i = 0; i < V; i++) {
@@ -289,10 +291,8 @@ template <typename T, bool E4M3, int N, int E, bool WARP> __global__ void __laun
       float y[N];
       load_weights<T, N>(a.weight, c, a.weight_f32, y);
 #pragma unroll
-      for (int j = 0; j < N; j++) y[j] = to_float(s[i].t[j]) * rstd * y[j];
+      for (int j = 0; j < N; j++) y[j] = to_float(s[i].t[j]) * factor * y[j];
       if (E4M3) {
-#pragma unroll
-        for (int j = 0; j < N; j++) y[j] *= sc.inverse;
         store_e4m3<N>((__nv_fp8_storage_t *)a.out + row * a.C + c, y);
       } else {
 #pragma unroll
@@ -303,64 +303,97 @@ template <typename T, bool E4M3, int N, int E, bool WARP> __global__ void __laun
   }
 }
 
-// Backward: the blocks walk over the rows; a thread's channels stay the same, and their weight gradients in its registers.
-template <typename T, int N, int E, bool WARP> __global__ void __launch_bounds__(WARP ? 256 : 512) norm_rows_grad_kernel(NormGradArgs a) {
-  constexpr int V = E / N;
+// Backward: the blocks walk over the rows; a thread's channels stay the same, and their weights and weight gradients in its
+// registers.  AHEAD: the next rows are on their way into shared memory, where every thread reads what it has copied itself.
+constexpr int kRowStages = 3;
+template <typename T, int N, int E, bool WARP, bool ADD, bool AHEAD>
+__global__ void __launch_bounds__(WARP ? 256 : 512, E == 8 ? (WARP ? 4 : 2) : 1) norm_rows_grad_kernel(NormGradArgs a) {
+  constexpr int V = E / N, TENSORS = ADD ? 3 : 2;
+  extern __shared__ __align__(16) unsigned char row_memory[];
   __shared__ float shared[2][32];
   __shared__ float sums[WARP ? 1024 : 1];
   const int threads = WARP ? 32 : (int)blockDim.x, thread = WARP ? threadIdx.x & 31 : threadIdx.x;
   const int64_t first = WARP ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x, step = WARP ? (int64_t)gridDim.x * 8 : gridDim.x;
-  float gw[V][N];
+  uint4 *slots = (uint4 *)row_memory + threadIdx.x;  // (stage, tensor, piece) x threads of the block
+  const auto slot = [&](int stage, int tensor, int i) { return slots + ((stage * TENSORS + tensor) * V + i) * (int)blockDim.x; };
+  const auto copy = [&](int64_t row, int stage) {
+    if (row < a.outer) {
 #pragma unroll
-  for (int i = 0; i < V; i++)
+      for (int i = 0; i < V; i++) {
+        const int c = (thread + i * threads) * N;
+        if (c < a.C) {
+          copy_16(slot(stage, 0, i), (const T *)a.s + row * a.s_stride + c);
+          copy_16(slot(stage, 1, i), (const T *)a.gout + row * a.C + c);
+          if (ADD) copy_16(slot(stage, 2, i), (const T *)a.gsum + row * a.C + c);
+        }
+      }
+    }
+    copies_end();
+  };
+  float w[V][N], gw[V][N];
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    const int c = (thread + i * threads) * N;
+    if (c < a.C) load_weights<T, N>(a.weight, c, a.weight_f32, w[i]);
 #pragma unroll
     for (int j = 0; j < N; j++) gw[i][j] = 0.f;
-  int turn = 0;
+  }
+  if (AHEAD)
+    for (int d = 0; d < kRowStages - 1; d++) copy(first + d * step, d);
+  int turn = 0, stage = 0;
+  float rstd_next = first < a.outer ? a.rstd[first] : 0.f;
   for (int64_t row = first; row < a.outer; row += step, turn ^= 1) {
-    const T *s_at = (const T *)a.s + row * a.s_stride, *g_at = (const T *)a.gout + row * a.C, *p_at = (const T *)a.gsum + row * a.C;
+    const float rstd = rstd_next;
+    if (row + step < a.outer) rstd_next = a.rstd[row + step];
     Piece<T, N> s[V], g[V], p[V];
+    if (AHEAD) {
+      copy(row + (kRowStages - 1) * step, stage == 0 ? kRowStages - 1 : stage - 1);
+      copies_wait<kRowStages - 1>();
+    }
 #pragma unroll
     for (int i = 0; i < V; i++) {
       const int c = (thread + i * threads) * N;
       if (c < a.C) {
-        s[i].load(s_at + c);
-        g[i].load(g_at + c);
-        if (a.gsum && a.gx) p[i].load(p_at + c);
+        if (AHEAD) {
+          s[i].load((const T *)slot(stage, 0, i));
+          g[i].load((const T *)slot(stage, 1, i));
+        } else {
+          s[i].load((const T *)a.s + row * a.s_stride + c);
+          g[i].load((const T *)a.gout + row * a.C + c);
+          if (ADD) p[i].load((const T *)a.gsum + row * a.C + c);
+        }
       }
     }
-    const float rstd = a.rstd[row];
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < V; i++) {
       const int c = (thread + i * threads) * N;
       if (c < a.C) {
-        float w[N];
-        load_weights<T, N>(a.weight, c, a.weight_f32, w);
 #pragma unroll
         for (int j = 0; j < N; j++) {
           const float gu = to_float(g[i].t[j]) * (to_float(s[i].t[j]) * rstd);
           gw[i][j] += gu;
-          dot = fmaf(gu, w[j], dot);
+          dot = fmaf(gu, w[i][j], dot);
         }
       }
     }
-    if (!a.gx) continue;
-    dot = row_sum<WARP>(dot, shared[turn]) * a.inv_c;
+    if (a.gx) {
+      dot = row_sum<WARP>(dot, shared[turn]) * (-rstd * rstd * a.inv_c);
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-      const int c = (thread + i * threads) * N;
-      if (c < a.C) {
-        float w[N];
-        load_weights<T, N>(a.weight, c, a.weight_f32, w);
+      for (int i = 0; i < V; i++) {
+        const int c = (thread + i * threads) * N;
+        if (c < a.C) {
+          if (AHEAD && ADD) p[i].load((const T *)slot(stage, 2, i));
 #pragma unroll
-        for (int j = 0; j < N; j++) {
-          float v = rstd * (to_float(g[i].t[j]) * w[j] - to_float(s[i].t[j]) * rstd * dot);
-          if (a.gsum) v += to_float(p[i].t[j]);
-          s[i].t[j] = from_float<T>(v);
+          for (int j = 0; j < N; j++) {
+            const float v = fmaf(to_float(g[i].t[j]) * w[i][j], rstd, to_float(s[i].t[j]) * dot);
+            s[i].t[j] = from_float<T>(ADD ? v + to_float(p[i].t[j]) : v);
+          }
+          s[i].store((T *)a.gx + row * a.C + c);
         }
-        s[i].store((T *)a.gx + row * a.C + c);
       }
     }
+    stage = stage == kRowStages - 1 ? 0 : stage + 1;
   }
   if (!a.gw) return;
   if (WARP) {  // the eight warps' sums, one after the other
@@ -398,17 +431,14 @@ template <typename T, bool E4M3, int N, int E> void norm_rows_launch(const NormA
   if (norm_path(a.C, 1) == kWarpRows)
     norm_rows_kernel<T, E4M3, N, E, true><<<(unsigned)((a.outer + 7) / 8), 256, 0, st>>>(a);
   else
-    norm_rows_kernel<T, E4M3, N, E, false><<<(unsigned)a.outer, 32 * cdiv(a.C, 32 * E), 0, st>>>(a);
+    norm_rows_kernel<T, E4M3, N, E, false><<<(unsigned)a.outer, norm_row_threads(a.C), 0, st>>>(a);
 }
-// Elements a thread holds: 32 a lane for up to 1024 in a warp; in blocks 8 where 512 threads are enough, 16, or 32.
 template <typename T, bool E4M3, int N> void norm_rows_pick(const NormArgs &a, cudaStream_t st) {
-  const int64_t per = norm_path(a.C, 1) == kWarpRows ? (a.C + 31) / 32 : (a.C + 511) / 512;
-  if (per <= 8)
-    norm_rows_launch<T, E4M3, N, 8>(a, st);
-  else if (per <= 16)
-    norm_rows_launch<T, E4M3, N, 16>(a, st);
-  else
-    norm_rows_launch<T, E4M3, N, 32>(a, st);
+  switch (norm_row_elements(a.C)) {
+    case 8: return norm_rows_launch<T, E4M3, N, 8>(a, st);
+    case 16: return norm_rows_launch<T, E4M3, N, 16>(a, st);
+    default: return norm_rows_launch<T, E4M3, N, 32>(a, st);
+  }
 }
 
 template <typename T, bool E4M3> void norm_launch(const NormArgs &a, cudaStream_t st) {
@@ -430,21 +460,28 @@ template <typename T, bool E4M3> void norm_launch(const NormArgs &a, cudaStream_
   }
 }
 
-template <typename T, int N, int E> void norm_rows_grad_launch(const NormGradArgs &a, cudaStream_t st) {
-  if (norm_path(a.C, 1) == kWarpRows)
-    norm_rows_grad_kernel<T, N, E, true><<<a.splits, 256, 0, st>>>(a);
-  else
-    norm_rows_grad_kernel<T, N, E, false><<<a.splits, 32 * cdiv(a.C, 32 * E), 0, st>>>(a);
+template <typename T, int N, int E, bool WARP> void norm_rows_grad_launch(const NormGradArgs &a, cudaStream_t st) {
+  const int threads = WARP ? 256 : norm_row_threads(a.C), tensors = a.gsum ? 3 : 2;
+  const int bytes = kRowStages * tensors * E * (int)sizeof(T) * threads;
+  if constexpr (N > 1) {
+    if (bytes <= kMostRowStages) {
+      void (*kernel)(NormGradArgs) = a.gsum ? norm_rows_grad_kernel<T, N, E, WARP, true, true> : norm_rows_grad_kernel<T, N, E, WARP, false, true>;
+      if (bytes > 32768) cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+      kernel<<<a.splits, threads, bytes, st>>>(a);
+      return;
+    }
+  }
+  (a.gsum ? norm_rows_grad_kernel<T, N, E, WARP, true, false> : norm_rows_grad_kernel<T, N, E, WARP, false, false>)<<<a.splits, threads, 0, st>>>(a);
 }
 template <typename T, int N> void norm_rows_grad_pick(const NormGradArgs &a, cudaStream_t st) {
-  const int64_t per = norm_path(a.C, 1) == kWarpRows ? (a.C + 31) / 32 : (a.C + 511) / 512;
-  if (per <= 8)
-    norm_rows_grad_launch<T, N, 8>(a, st);
-  else if (per <= 16)
-    norm_rows_grad_launch<T, N, 16>(a, st);
-  else
-    norm_rows_grad_launch<T, N, 32>(a, st);
+  const bool warp = norm_path(a.C, 1) == kWarpRows;
+  switch (norm_row_elements(a.C)) {
+    case 8: return warp ? norm_rows_grad_launch<T, N, 8, true>(a, st) : norm_rows_grad_launch<T, N, 8, false>(a, st);
+    case 16: return warp ? norm_rows_grad_launch<T, N, 16, true>(a, st) : norm_rows_grad_launch<T, N, 16, false>(a, st);
+    default: return warp ? norm_rows_grad_launch<T, N, 32, true>(a, st) : norm_rows_grad_launch<T, N, 32, false>(a, st);
+  }
 }
+
 // Kernels launched.
 template <typename T> int norm_grad_launch(NormGradArgs &a, cudaStream_t st) {
   constexpr int N = 16 / (int)sizeof(T);

@@ -10,6 +10,8 @@
 // gradient is that of the function computed.
 #pragma once
 
+#include <algorithm>
+
 #include "element.cuh"
 
 namespace sph {
@@ -40,12 +42,22 @@ enum NormPath { kLongRows, kWarpRows, kBlockRows, kPlanes, kDeepPlanes };
 inline NormPath norm_path(int64_t C, int64_t inner) {
   return inner > 1 ? (C <= 512 ? kPlanes : kDeepPlanes) : C <= 1024 ? kWarpRows : C <= 16384 ? kBlockRows : kLongRows;
 }
+// Rows in registers: elements a thread holds (32 a lane are the 1024 of a warp, blocks have up to 512 threads), and the threads
+// of a block that has a row.
+inline int norm_row_elements(int64_t C) {
+  const int64_t per = C <= 1024 ? (C + 31) / 32 : (C + 511) / 512;
+  return per <= 8 ? 8 : per <= 16 ? 16 : 32;
+}
+inline int norm_row_threads(int64_t C) { return 32 * cdiv(C, 32 * norm_row_elements(C)); }
+// Shared memory that a block may have for the rows ahead.
+constexpr int kMostRowStages = 216 * 1024;
 inline int norm_splits(int64_t outer, int64_t C, int64_t inner) {
   const int64_t norms = outer * inner;
   int64_t want, most;
   switch (norm_path(C, inner)) {
-    case kWarpRows: want = 148 * 4, most = (norms + 7) / 8; break;
-    case kBlockRows: want = 148 * 3, most = norms; break;
+    // as many blocks as are on the SMs at once
+    case kWarpRows: want = 148 * (norm_row_elements(C) == 8 ? 4 : 1), most = (norms + 7) / 8; break;
+    case kBlockRows: want = 148 * std::max(1, (norm_row_elements(C) == 8 ? 1024 : 512) / norm_row_threads(C)), most = norms; break;
     case kPlanes: want = 148 * 3, most = (norms + 31) / 32; break;
     default: {
       const int64_t blocks = inner == 1 ? (C + 31) / 32 : C;  // enough blocks for the GPU, at least 64 norms each

@@ -25,9 +25,9 @@ template <typename T, bool E4M3, bool ADD, int MODE, int LOG> __global__ void __
   const T *other = ADD ? add + first * G::PITCH + px.col + (MODE == kShifted ? shift_of((const T *)a.residual + run.offset(0), 0, first, a.inner) : 0) : nullptr;
   copies_wait<0>();
   __syncthreads();
-  float v[N];
+  float v[N], most[N];  // sums of squares; largest |s w|
 #pragma unroll
-  for (int i = 0; i < N; i++) v[i] = 0.f;
+  for (int i = 0; i < N; i++) v[i] = most[i] = 0.f;
   {
     T *p = mine;
     int64_t plane = 0;
@@ -42,33 +42,24 @@ template <typename T, bool E4M3, bool ADD, int MODE, int LOG> __global__ void __
         px.store((T *)a.sum, plane, q);
       }
 #pragma unroll
-      for (int i = 0; i < N; i++) v[i] = fmaf(to_float(q.t[i]), to_float(q.t[i]), v[i]);
+      for (int i = 0; i < N; i++) {
+        const float f = to_float(q.t[i]);
+        v[i] = fmaf(f, f, v[i]);
+        if (E4M3) most[i] = max_nan(most[i], fabsf(f * weight[c]));
+      }
     }
   }
   plane_join<LOG>(v, shared[0], [](float p, float q) { return p + q; });
+  if (E4M3) plane_join<LOG>(most, shared[1], [](float p, float q) { return max_nan(p, q); });
   float rstd[N], scale[N];
 #pragma unroll
   for (int i = 0; i < N; i++) {
     rstd[i] = 1.f / sqrtf(v[i] * a.inv_c + a.eps);
     if (first == 0 && px.in[i] && a.rstd) a.rstd[px.norm[i]] = rstd[i];
-    scale[i] = 1.f;
-  }
-  if (E4M3) {
-#pragma unroll
-    for (int i = 0; i < N; i++) v[i] = 0.f;
-    const T *p = mine;
-#pragma unroll 8
-    for (int c = first; c < a.C; c += ACROSS, p += G::ROW) {
-      const Pixels<T> q = L::load(p);
-#pragma unroll
-      for (int i = 0; i < N; i++) v[i] = max_nan(v[i], fabsf(to_float(q.t[i]) * rstd[i] * weight[c]));
-    }
-    plane_join<LOG>(v, shared[1], [](float p, float q) { return max_nan(p, q); });
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-      const Scale sc = Scale::of(v[i]);
-      scale[i] = sc.inverse;
+    if (E4M3) {
+      const Scale sc = Scale::of(most[i] * rstd[i]);
       if (first == 0 && px.in[i]) a.scale[px.norm[i]] = sc.scale;
+      scale[i] = rstd[i] * sc.inverse;
     }
   }
   const T *p = mine;
@@ -78,10 +69,8 @@ template <typename T, bool E4M3, bool ADD, int MODE, int LOG> __global__ void __
     Pixels<T> q = L::load(p);
     float y[N];
 #pragma unroll
-    for (int i = 0; i < N; i++) y[i] = to_float(q.t[i]) * rstd[i] * weight[c];
+    for (int i = 0; i < N; i++) y[i] = to_float(q.t[i]) * (E4M3 ? scale[i] : rstd[i]) * weight[c];
     if (E4M3) {
-#pragma unroll
-      for (int i = 0; i < N; i++) y[i] *= scale[i];
       px.store_e4m3((__nv_fp8_storage_t *)a.out, plane, y);
     } else {
 #pragma unroll

@@ -77,15 +77,6 @@ template <int MODE, int PIXELS> struct Run {
   }
 };
 
-__device__ __forceinline__ void copy_16(void *to, const void *from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copy_4(void *to, const void *from) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int PENDING> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
-
 // Elements between the 16-byte boundary before a channel's run and the run (kShifted), the same for a warp's channels.
 template <typename T> __device__ __forceinline__ int shift_of(const T *from, int64_t offset, int c, int64_t inner) {
   return (int)(((uintptr_t)(from + offset) / sizeof(T) + (uintptr_t)c * (uintptr_t)inner) & (Pixels<T>::V - 1));
@@ -162,9 +153,11 @@ template <typename T, int MODE, int LOG> struct Lane {
     for (int i = 0; i < N; i++) {
       in[i] = run.has(col + i * STEP);
       norm[i] = run.norm(col + i * STEP);
-      off[i] = in[i] && (MODE != kWide || i == 0) ? run.offset(col + i * STEP) + first * run.inner : 0;
+      off[i] = in[i] && (MODE == kSingle || i == 0) ? run.offset(col + i * STEP) + first * run.inner : 0;
     }
   }
+  // (The pixels of a shifted run are in one image.)
+  __device__ __forceinline__ int64_t at(int i) const { return MODE == kShifted ? off[0] + i * STEP : off[i]; }
   static __device__ __forceinline__ Pixels<T> load(const T *p) {
     Pixels<T> v;
     if (MODE == kWide) v.w = *(const unsigned *)p;
@@ -188,7 +181,7 @@ template <typename T, int MODE, int LOG> struct Lane {
     } else {
 #pragma unroll
       for (int i = 0; i < N; i++)
-        if (in[i]) to[off[i] + plane] = v.t[i];
+        if (in[i]) to[at(i) + plane] = v.t[i];
     }
   }
   __device__ __forceinline__ void store_e4m3(__nv_fp8_storage_t *to, int64_t plane, const float (&y)[N]) const {
@@ -199,7 +192,7 @@ template <typename T, int MODE, int LOG> struct Lane {
     } else {
 #pragma unroll
       for (int i = 0; i < N; i++)
-        if (in[i]) to[off[i] + plane] = to_e4m3(y[i]);
+        if (in[i]) to[at(i) + plane] = to_e4m3(y[i]);
     }
   }
 };
