@@ -24,7 +24,7 @@ OBJ = os.path.join(HERE, "build", "obj")
 INCLUDE = os.path.join(ROOT, "include")
 
 CU_SOURCES = ["resample.cu", "plan.cu", "pool.cu", "maps.cu", "conv.cu", "conv_simt.cu", "conv_small.cu", "conv_tc.cu", "conv_x3.cu",
-              "norm.cu", "norm_planes.cu", "norm_planes_grad.cu", "log_probs.cu", "adamw.cu"]
+              "norm.cu", "norm_flat.cu", "norm_planes.cu", "norm_planes_grad.cu", "log_probs.cu", "adamw.cu"]
 SHIM_SOURCES = ["torch_shim.cpp", "torch_shim_net.cpp"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--extended-lambda",
               "-Xcompiler", "-fPIC", "-I" + INCLUDE, "-I" + CSRC]

@@ -60,6 +60,11 @@ template <class F> __device__ __forceinline__ float warp_join(float v, F f) {
   for (int d = 16; d > 0; d >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, d));
   return v;
 }
+// Over groups of `lanes` neighbouring lanes, a power of two.
+template <class F> __device__ __forceinline__ float lanes_join(float v, int lanes, F f) {
+  for (int d = lanes >> 1; d > 0; d >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, d));
+  return v;
+}
 __device__ __forceinline__ float warp_sum(float v) {
   return warp_join(v, [](float a, float b) { return a + b; });
 }

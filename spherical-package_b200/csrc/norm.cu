@@ -1,8 +1,6 @@
 // Norms over rows and over planes of many channels; see norm.cuh for the formulas.
 #include "norm.cuh"
 
-#include <type_traits>
-
 namespace sph {
 
 // One block per row (inner == 1).
@@ -220,100 +218,134 @@ template <typename T, int N> __device__ __forceinline__ void load_weights(const 
   }
 }
 
-// Joins over the threads of a row: a warp, or the whole block (`shared`: 32 floats, not those of the join before).
-template <bool WARP, class F> __device__ __forceinline__ float row_join(float v, float *shared, F f, float none) {
+// Joins over the threads of a row: `lanes` of a warp (a power of two), or the whole block (`shared`: 32 floats, not those of the
+// join before).
+template <bool WARP, class F> __device__ __forceinline__ float row_join(float v, float *shared, F f, float none, int lanes) {
+  if (WARP) return lanes_join(v, lanes, f);
   v = warp_join(v, f);
-  if (WARP) return v;
   const int lane = threadIdx.x & 31;
   if (lane == 0) shared[threadIdx.x >> 5] = v;
   __syncthreads();
   return warp_join(lane < (int)(blockDim.x >> 5) ? shared[lane] : none, f);
 }
-template <bool WARP> __device__ __forceinline__ float row_sum(float v, float *shared) {
-  return row_join<WARP>(v, shared, [](float p, float q) { return p + q; }, 0.f);
+template <bool WARP> __device__ __forceinline__ float row_sum(float v, float *shared, int lanes) {
+  return row_join<WARP>(v, shared, [](float p, float q) { return p + q; }, 0.f, lanes);
 }
 
 // A row is held by a warp (WARP) or by a block, E elements a thread in pieces of N: every tensor is read and written once.
-template <typename T, bool E4M3, int N, int E, bool WARP> __global__ void __launch_bounds__(WARP ? 256 : 512) norm_rows_kernel(NormArgs a) {
+// AHEAD: the blocks walk over the rows, and the next ones are on their way into shared memory, where every thread reads what it
+// has copied itself.
+constexpr int kRowStages = 3;
+template <typename T, bool E4M3, int N, int E, bool WARP, bool AHEAD>
+__global__ void __launch_bounds__(WARP ? 256 : 512, AHEAD && E == 8 ? (WARP ? 4 : 2) : 1) norm_rows_kernel(NormArgs a) {
   constexpr int V = E / N;
-  __shared__ float shared[2][32];
-  const int threads = WARP ? 32 : (int)blockDim.x, thread = WARP ? threadIdx.x & 31 : threadIdx.x;
-  const int64_t row = WARP ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
-  if (WARP && row >= a.outer) return;
-  const T *x = (const T *)a.x + row * a.x_stride, *r = a.residual ? (const T *)a.residual + row * a.r_stride : nullptr;
-  Piece<T, N> s[V], add[V];
+  extern __shared__ __align__(16) unsigned char row_memory[];
+  __shared__ float shared[2][2][32];
+  const int threads = WARP ? a.lanes : (int)blockDim.x, thread = WARP ? threadIdx.x & (threads - 1) : threadIdx.x, lane = threadIdx.x & 31;
+  const int each = WARP ? 256 / threads : 1;  // rows of a block at once
+  const int64_t first = WARP ? (int64_t)blockIdx.x * each + threadIdx.x / threads : blockIdx.x, step = (int64_t)gridDim.x * each;
+  const int tensors = a.residual ? 2 : 1;
+  const auto slot = [&](int stage, int tensor, int i) {
+    return (uint4 *)row_memory + threadIdx.x + ((stage * tensors + tensor) * V + i) * (int)blockDim.x;
+  };
+  const auto copy = [&](int64_t row, int stage) {
+    if (row < a.outer) {
 #pragma unroll
-  for (int i = 0; i < V; i++) {
-    const int c = (thread + i * threads) * N;
-    if (c < a.C) {
-      s[i].load(x + c);
-      if (r) add[i].load(r + c);
-    }
-  }
-  float sq = 0.f, most = 0.f;  // sum of squares; largest |s w|
-#pragma unroll
-  for (int i = 0; i < V; i++) {
-    const int c = (thread + i * threads) * N;
-    if (c < a.C) {
-      if (r) {
-#pragma unroll
-        for (int j = 0; j < N; j++) s[i].t[j] = from_float<T>(to_float(s[i].t[j]) + to_float(add[i].t[j]));
-        s[i].store((T *)a.sum + row * a.C + c);
-      }
-      float w[N];
-      if (E4M3) load_weights<T, N>(a.weight, c, a.weight_f32, w);
-#pragma unroll
-      for (int j = 0; j < N; j++) {
-        const float f = to_float(s[i].t[j]);
-        sq = fmaf(f, f, sq);
-        if (E4M3) most = max_nan(most, fabsf(f * w[j]));
+      for (int i = 0; i < V; i++) {
+        const int c = (thread + i * threads) * N;
+        if (c < a.C) {
+          copy_16(slot(stage, 0, i), (const T *)a.x + row * a.x_stride + c);
+          if (a.residual) copy_16(slot(stage, 1, i), (const T *)a.residual + row * a.r_stride + c);
+        }
       }
     }
-  }
-  if (E4M3) {  // both joins behind one barrier
-    most = warp_join(most, [](float p, float q) { return max_nan(p, q); });
-    if (!WARP && (threadIdx.x & 31) == 0) shared[1][threadIdx.x >> 5] = most;
-  }
-  const float rstd = 1.f / sqrtf(row_sum<WARP>(sq, shared[0]) * a.inv_c + a.eps);
-  if (thread == 0 && a.rstd) a.rstd[row] = rstd;
-  float factor = rstd;
-  if (E4M3) {
-    const int lane = threadIdx.x & 31;
-    if (!WARP) most = warp_join(lane < (int)(blockDim.x >> 5) ? shared[1][lane] : 0.f, [](float p, float q) { return max_nan(p, q); });
-    const Scale sc = Scale::of(most * rstd);
-    if (thread == 0) a.scale[row] = sc.scale;
-    factor *= sc.inverse;
-  }
+    copies_end();
+  };
+  if (AHEAD)
+    for (int d = 0; d < kRowStages - 1; d++) copy(first + d * step, d);
+  int turn = 0, stage = 0;
+  // (the lanes of a warp stay together: those past the last row work on nothing)
+  for (int64_t row = first; row - (WARP ? lane / threads : 0) < a.outer; row += step, turn ^= 1) {
+    const int C = !WARP || row < a.outer ? a.C : 0;
+    Piece<T, N> s[V], add[V];
+    if (AHEAD) {
+      copy(row + (kRowStages - 1) * step, stage == 0 ? kRowStages - 1 : stage - 1);
+      copies_wait<kRowStages - 1>();
+    }
 #pragma unroll
-  for (int i = 0; i < V; i++) {
-    const int c = (thread + i * threads) * N;
-    if (c < a.C) {
-      float y[N];
-      load_weights<T, N>(a.weight, c, a.weight_f32, y);
-#pragma unroll
-      for (int j = 0; j < N; j++) y[j] = to_float(s[i].t[j]) * factor * y[j];
-      if (E4M3) {
-        store_e4m3<N>((__nv_fp8_storage_t *)a.out + row * a.C + c, y);
-      } else {
-#pragma unroll
-        for (int j = 0; j < N; j++) s[i].t[j] = from_float<T>(y[j]);
-        s[i].store((T *)a.out + row * a.C + c);
+    for (int i = 0; i < V; i++) {
+      const int c = (thread + i * threads) * N;
+      if (c < C) {
+        s[i].load(AHEAD ? (const T *)slot(stage, 0, i) : (const T *)a.x + row * a.x_stride + c);
+        if (a.residual) add[i].load(AHEAD ? (const T *)slot(stage, 1, i) : (const T *)a.residual + row * a.r_stride + c);
       }
     }
+    float sq = 0.f, most = 0.f;  // sum of squares; largest |s w|
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      const int c = (thread + i * threads) * N;
+      if (c < C) {
+        if (a.residual) {
+#pragma unroll
+          for (int j = 0; j < N; j++) s[i].t[j] = from_float<T>(to_float(s[i].t[j]) + to_float(add[i].t[j]));
+          s[i].store((T *)a.sum + row * a.C + c);
+        }
+        float w[N];
+        if (E4M3) load_weights<T, N>(a.weight, c, a.weight_f32, w);
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+          const float f = to_float(s[i].t[j]);
+          sq = fmaf(f, f, sq);
+          if (E4M3) most = max_nan(most, fabsf(f * w[j]));
+        }
+      }
+    }
+    if (E4M3) {  // both joins behind one barrier
+      most = lanes_join(most, WARP ? threads : 32, [](float p, float q) { return max_nan(p, q); });
+      if (!WARP && lane == 0) shared[turn][1][threadIdx.x >> 5] = most;
+    }
+    const float rstd = 1.f / sqrtf(row_sum<WARP>(sq, shared[turn][0], threads) * a.inv_c + a.eps);
+    if (thread == 0 && a.rstd && C) a.rstd[row] = rstd;
+    float factor = rstd;
+    if (E4M3) {
+      if (!WARP)
+        most = warp_join(lane < (int)(blockDim.x >> 5) ? shared[turn][1][lane] : 0.f, [](float p, float q) { return max_nan(p, q); });
+      const Scale sc = Scale::of(most * rstd);
+      if (thread == 0 && C) a.scale[row] = sc.scale;
+      factor *= sc.inverse;
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      const int c = (thread + i * threads) * N;
+      if (c < C) {
+        float y[N];
+        load_weights<T, N>(a.weight, c, a.weight_f32, y);
+#pragma unroll
+        for (int j = 0; j < N; j++) y[j] = to_float(s[i].t[j]) * factor * y[j];
+        if (E4M3) {
+          store_e4m3<N>((__nv_fp8_storage_t *)a.out + row * a.C + c, y);
+        } else {
+#pragma unroll
+          for (int j = 0; j < N; j++) s[i].t[j] = from_float<T>(y[j]);
+          s[i].store((T *)a.out + row * a.C + c);
+        }
+      }
+    }
+    stage = stage == kRowStages - 1 ? 0 : stage + 1;
   }
 }
 
 // Backward: the blocks walk over the rows; a thread's channels stay the same, and their weights and weight gradients in its
-// registers.  AHEAD: the next rows are on their way into shared memory, where every thread reads what it has copied itself.
-constexpr int kRowStages = 3;
+// registers.
 template <typename T, int N, int E, bool WARP, bool ADD, bool AHEAD>
 __global__ void __launch_bounds__(WARP ? 256 : 512, E == 8 ? (WARP ? 4 : 2) : 1) norm_rows_grad_kernel(NormGradArgs a) {
   constexpr int V = E / N, TENSORS = ADD ? 3 : 2;
   extern __shared__ __align__(16) unsigned char row_memory[];
   __shared__ float shared[2][32];
   __shared__ float sums[WARP ? 1024 : 1];
-  const int threads = WARP ? 32 : (int)blockDim.x, thread = WARP ? threadIdx.x & 31 : threadIdx.x;
-  const int64_t first = WARP ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x, step = WARP ? (int64_t)gridDim.x * 8 : gridDim.x;
+  const int threads = WARP ? a.lanes : (int)blockDim.x, thread = WARP ? threadIdx.x & (threads - 1) : threadIdx.x, lane = threadIdx.x & 31;
+  const int each = WARP ? 256 / threads : 1;  // rows of a block at once
+  const int64_t first = WARP ? (int64_t)blockIdx.x * each + threadIdx.x / threads : blockIdx.x, step = (int64_t)gridDim.x * each;
   uint4 *slots = (uint4 *)row_memory + threadIdx.x;  // (stage, tensor, piece) x threads of the block
   const auto slot = [&](int stage, int tensor, int i) { return slots + ((stage * TENSORS + tensor) * V + i) * (int)blockDim.x; };
   const auto copy = [&](int64_t row, int stage) {
@@ -342,7 +374,8 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, E == 8 ? (WARP ? 4 : 2) : 1)
     for (int d = 0; d < kRowStages - 1; d++) copy(first + d * step, d);
   int turn = 0, stage = 0;
   float rstd_next = first < a.outer ? a.rstd[first] : 0.f;
-  for (int64_t row = first; row < a.outer; row += step, turn ^= 1) {
+  for (int64_t row = first; row - (WARP ? lane / threads : 0) < a.outer; row += step, turn ^= 1) {
+    const int C = !WARP || row < a.outer ? a.C : 0;
     const float rstd = rstd_next;
     if (row + step < a.outer) rstd_next = a.rstd[row + step];
     Piece<T, N> s[V], g[V], p[V];
@@ -353,7 +386,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, E == 8 ? (WARP ? 4 : 2) : 1)
 #pragma unroll
     for (int i = 0; i < V; i++) {
       const int c = (thread + i * threads) * N;
-      if (c < a.C) {
+      if (c < C) {
         if (AHEAD) {
           s[i].load((const T *)slot(stage, 0, i));
           g[i].load((const T *)slot(stage, 1, i));
@@ -368,7 +401,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, E == 8 ? (WARP ? 4 : 2) : 1)
 #pragma unroll
     for (int i = 0; i < V; i++) {
       const int c = (thread + i * threads) * N;
-      if (c < a.C) {
+      if (c < C) {
 #pragma unroll
         for (int j = 0; j < N; j++) {
           const float gu = to_float(g[i].t[j]) * (to_float(s[i].t[j]) * rstd);
@@ -378,11 +411,11 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, E == 8 ? (WARP ? 4 : 2) : 1)
       }
     }
     if (a.gx) {
-      dot = row_sum<WARP>(dot, shared[turn]) * (-rstd * rstd * a.inv_c);
+      dot = row_sum<WARP>(dot, shared[turn], threads) * (-rstd * rstd * a.inv_c);
 #pragma unroll
       for (int i = 0; i < V; i++) {
         const int c = (thread + i * threads) * N;
-        if (c < a.C) {
+        if (c < C) {
           if (AHEAD && ADD) p[i].load((const T *)slot(stage, 2, i));
 #pragma unroll
           for (int j = 0; j < N; j++) {
@@ -396,16 +429,21 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, E == 8 ? (WARP ? 4 : 2) : 1)
     stage = stage == kRowStages - 1 ? 0 : stage + 1;
   }
   if (!a.gw) return;
-  if (WARP) {  // the eight warps' sums, one after the other
+  if (WARP) {  // the rows' sums in each warp, and the eight warps' sums, one after the other
+#pragma unroll
+    for (int i = 0; i < V; i++)
+#pragma unroll
+      for (int j = 0; j < N; j++)
+        for (int d = threads; d < 32; d <<= 1) gw[i][j] += __shfl_xor_sync(0xffffffffu, gw[i][j], d);
     for (int c = threadIdx.x; c < a.C; c += 256) sums[c] = 0.f;
-    for (int w = 0; w < 8; w++) {
+    for (int k = 0; k < 8; k++) {
       __syncthreads();
-      if ((int)(threadIdx.x >> 5) == w)
+      if ((int)(threadIdx.x >> 5) == k && lane < threads)
 #pragma unroll
         for (int i = 0; i < V; i++)
 #pragma unroll
           for (int j = 0; j < N; j++) {
-            const int c = (thread + i * 32) * N + j;
+            const int c = (thread + i * threads) * N + j;
             if (c < a.C) sums[c] += gw[i][j];
           }
     }
@@ -427,21 +465,33 @@ inline bool rows_aligned(const void *p, int64_t stride, size_t size) {
   return (uintptr_t)p % 16 == 0 && stride * (int64_t)size % 16 == 0;
 }
 
-template <typename T, bool E4M3, int N, int E> void norm_rows_launch(const NormArgs &a, cudaStream_t st) {
-  if (norm_path(a.C, 1) == kWarpRows)
-    norm_rows_kernel<T, E4M3, N, E, true><<<(unsigned)((a.outer + 7) / 8), 256, 0, st>>>(a);
-  else
-    norm_rows_kernel<T, E4M3, N, E, false><<<(unsigned)a.outer, norm_row_threads(a.C), 0, st>>>(a);
+template <typename T, bool E4M3, int N, int E, bool WARP> void norm_rows_launch(const NormArgs &a, cudaStream_t st) {
+  const int threads = WARP ? 256 : norm_row_threads(a.C), each = WARP ? 256 / a.lanes : 1;
+  const int bytes = kRowStages * (a.residual ? 2 : 1) * E * (int)sizeof(T) * threads;
+  const int64_t blocks = (a.outer + each - 1) / each;
+  if constexpr (N > 1 && !WARP) {
+    // Copying ahead pays from four rows a block on; the blocks are as many as there is room for on the SMs.
+    const int fit = std::min((E == 8 ? 1024 : 512) / threads, 220 * 1024 / (bytes + 2048));
+    if (fit >= 1 && blocks >= 4 * 148 * fit) {
+      if (bytes > 32768)
+        cudaFuncSetAttribute((const void *)norm_rows_kernel<T, E4M3, N, E, WARP, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+      norm_rows_kernel<T, E4M3, N, E, WARP, true><<<148 * fit, threads, bytes, st>>>(a);
+      return;
+    }
+  }
+  norm_rows_kernel<T, E4M3, N, E, WARP, false><<<(unsigned)blocks, threads, 0, st>>>(a);
 }
-template <typename T, bool E4M3, int N> void norm_rows_pick(const NormArgs &a, cudaStream_t st) {
+template <typename T, bool E4M3, int N> void norm_rows_pick(NormArgs a, cudaStream_t st) {
+  const bool warp = norm_path(a.C, 1) == kWarpRows;
+  a.lanes = norm_row_lanes(a.C);
   switch (norm_row_elements(a.C)) {
-    case 8: return norm_rows_launch<T, E4M3, N, 8>(a, st);
-    case 16: return norm_rows_launch<T, E4M3, N, 16>(a, st);
-    default: return norm_rows_launch<T, E4M3, N, 32>(a, st);
+    case 8: return warp ? norm_rows_launch<T, E4M3, N, 8, true>(a, st) : norm_rows_launch<T, E4M3, N, 8, false>(a, st);
+    case 16: return warp ? norm_rows_launch<T, E4M3, N, 16, true>(a, st) : norm_rows_launch<T, E4M3, N, 16, false>(a, st);
+    default: return warp ? norm_rows_launch<T, E4M3, N, 32, true>(a, st) : norm_rows_launch<T, E4M3, N, 32, false>(a, st);
   }
 }
 
-template <typename T, bool E4M3> void norm_launch(const NormArgs &a, cudaStream_t st) {
+template <typename T, bool E4M3> void norm_launch(const NormArgs &a, int dtype, cudaStream_t st) {
   constexpr int N = 16 / (int)sizeof(T);
   switch (norm_path(a.C, a.inner)) {
     case kWarpRows:
@@ -449,18 +499,19 @@ template <typename T, bool E4M3> void norm_launch(const NormArgs &a, cudaStream_
       if (rows_aligned(a.x, a.x_stride, sizeof(T)) && a.C % N == 0 && rows_aligned(a.residual, a.r_stride, sizeof(T)) &&
           ((uintptr_t)a.sum % 16 | (uintptr_t)a.out % 16 | (uintptr_t)a.weight % 16) == 0)
         norm_rows_pick<T, E4M3, N>(a, st);
-      else
+      else if (!norm_flat_forward(a, dtype, st))
         norm_rows_pick<T, E4M3, 1>(a, st);
       break;
     case kPlanes:
-      norm_planes_forward(a, sizeof(T) == 4 ? SPH_F32 : std::is_same<T, __half>::value ? SPH_F16 : SPH_BF16, st);
+      norm_planes_forward(a, dtype, st);
       break;
     case kLongRows: norm_long_rows_kernel<T, E4M3><<<(unsigned)a.outer, 256, 0, st>>>(a); break;
     default: norm_deep_planes_kernel<T, E4M3><<<(unsigned)((a.outer * a.inner + 255) / 256), 256, 0, st>>>(a);
   }
 }
 
-template <typename T, int N, int E, bool WARP> void norm_rows_grad_launch(const NormGradArgs &a, cudaStream_t st) {
+template <typename T, int N, int E, bool WARP> void norm_rows_grad_launch(NormGradArgs &a, cudaStream_t st) {
+  a.splits = std::min(a.splits, 148 * (WARP ? (E == 8 ? 4 : E == 16 ? 2 : 1) : std::max(1, (E == 8 ? 1024 : 512) / norm_row_threads(a.C))));
   const int threads = WARP ? 256 : norm_row_threads(a.C), tensors = a.gsum ? 3 : 2;
   const int bytes = kRowStages * tensors * E * (int)sizeof(T) * threads;
   if constexpr (N > 1) {
@@ -473,8 +524,9 @@ template <typename T, int N, int E, bool WARP> void norm_rows_grad_launch(const 
   }
   (a.gsum ? norm_rows_grad_kernel<T, N, E, WARP, true, false> : norm_rows_grad_kernel<T, N, E, WARP, false, false>)<<<a.splits, threads, 0, st>>>(a);
 }
-template <typename T, int N> void norm_rows_grad_pick(const NormGradArgs &a, cudaStream_t st) {
+template <typename T, int N> void norm_rows_grad_pick(NormGradArgs &a, cudaStream_t st) {
   const bool warp = norm_path(a.C, 1) == kWarpRows;
+  a.lanes = norm_row_lanes(a.C);
   switch (norm_row_elements(a.C)) {
     case 8: return warp ? norm_rows_grad_launch<T, N, 8, true>(a, st) : norm_rows_grad_launch<T, N, 8, false>(a, st);
     case 16: return warp ? norm_rows_grad_launch<T, N, 16, true>(a, st) : norm_rows_grad_launch<T, N, 16, false>(a, st);
@@ -483,7 +535,7 @@ template <typename T, int N> void norm_rows_grad_pick(const NormGradArgs &a, cud
 }
 
 // Kernels launched.
-template <typename T> int norm_grad_launch(NormGradArgs &a, cudaStream_t st) {
+template <typename T> int norm_grad_launch(NormGradArgs &a, int dtype, cudaStream_t st) {
   constexpr int N = 16 / (int)sizeof(T);
   int launches = 0;
   if (a.outer > 0) {
@@ -494,11 +546,11 @@ template <typename T> int norm_grad_launch(NormGradArgs &a, cudaStream_t st) {
         if (rows_aligned(a.s, a.s_stride, sizeof(T)) && a.C % N == 0 &&
             ((uintptr_t)a.gout % 16 | (uintptr_t)a.gsum % 16 | (uintptr_t)a.gx % 16 | (uintptr_t)a.weight % 16) == 0)
           norm_rows_grad_pick<T, N>(a, st);
-        else
+        else if (!norm_flat_backward(a, dtype, st))
           norm_rows_grad_pick<T, 1>(a, st);
         break;
       case kPlanes:
-        norm_planes_backward(a, sizeof(T) == 4 ? SPH_F32 : std::is_same<T, __half>::value ? SPH_F16 : SPH_BF16, st);
+        norm_planes_backward(a, dtype, st);
         break;
       case kLongRows:
         if (a.gx) norm_long_rows_grad_kernel<T><<<(unsigned)a.outer, 256, 0, st>>>(a);
@@ -543,9 +595,9 @@ extern "C" int sph_rms_norm_forward(const void *x, const void *residual, const v
   cudaStream_t st = (cudaStream_t)stream;
   SPH_DISPATCH_ELEMENT(dtype, {
     if (scale)
-      norm_launch<T, true>(a, st);
+      norm_launch<T, true>(a, dtype, st);
     else
-      norm_launch<T, false>(a, st);
+      norm_launch<T, false>(a, dtype, st);
   });
   return launch_status();
 }
@@ -568,6 +620,6 @@ extern "C" int sph_rms_norm_backward(const void *gout, const void *gsum, const v
                        1.f / (float)C, weight_dtype == SPH_F32};
   cudaStream_t st = (cudaStream_t)stream;
   int launches = 0;
-  SPH_DISPATCH_ELEMENT(dtype, launches = norm_grad_launch<T>(a, st));
+  SPH_DISPATCH_ELEMENT(dtype, launches = norm_grad_launch<T>(a, dtype, st));
   return launch_status(launches);
 }

@@ -24,6 +24,7 @@ struct NormArgs {
   int C;
   float eps, inv_c;
   bool weight_f32;
+  int lanes;  // of a row that has a part of a warp
 };
 
 struct NormGradArgs {
@@ -35,6 +36,7 @@ struct NormGradArgs {
   int C, splits;
   float inv_c;
   bool weight_f32;
+  int lanes;  // of a row that has a part of a warp
 };
 
 // Which kernel takes a call, and in how many blocks its weight gradient is summed.
@@ -48,6 +50,12 @@ inline int norm_row_elements(int64_t C) {
   const int64_t per = C <= 1024 ? (C + 31) / 32 : (C + 511) / 512;
   return per <= 8 ? 8 : per <= 16 ? 16 : 32;
 }
+// Lanes of a warp that share a row, with up to eight elements each where the row has no more than 256.
+inline int norm_row_lanes(int64_t C) {
+  int n = 1;
+  while (n < 32 && (int64_t)8 * n < C) n *= 2;
+  return n;
+}
 inline int norm_row_threads(int64_t C) { return 32 * cdiv(C, 32 * norm_row_elements(C)); }
 // Shared memory that a block may have for the rows ahead.
 constexpr int kMostRowStages = 216 * 1024;
@@ -55,9 +63,9 @@ inline int norm_splits(int64_t outer, int64_t C, int64_t inner) {
   const int64_t norms = outer * inner;
   int64_t want, most;
   switch (norm_path(C, inner)) {
-    // as many blocks as are on the SMs at once
-    case kWarpRows: want = 148 * (norm_row_elements(C) == 8 ? 4 : 1), most = (norms + 7) / 8; break;
-    case kBlockRows: want = 148 * std::max(1, (norm_row_elements(C) == 8 ? 1024 : 512) / norm_row_threads(C)), most = norms; break;
+    // as many blocks as may be on the SMs at once; the launches take as many as are
+    case kWarpRows: want = 148 * 4, most = (norms + 7) / 8; break;
+    case kBlockRows: want = 148 * std::max(1, (norm_row_elements(C) <= 16 ? 1024 : 512) / norm_row_threads(C)), most = norms; break;
     case kPlanes: want = 148 * 3, most = (norms + 31) / 32; break;
     default: {
       const int64_t blocks = inner == 1 ? (C + 31) / 32 : C;  // enough blocks for the GPU, at least 64 norms each
@@ -72,5 +80,9 @@ inline int norm_splits(int64_t outer, int64_t C, int64_t inner) {
 void norm_planes_forward(const NormArgs &a, int dtype, cudaStream_t st);
 // (backward: may take fewer splits)
 void norm_planes_backward(NormGradArgs &a, int dtype, cudaStream_t st);
+
+// norm_flat.cu: rows of dense tensors that do not start on 16-byte boundaries; false where the tensors do not lie alike.
+bool norm_flat_forward(const NormArgs &a, int dtype, cudaStream_t st);
+bool norm_flat_backward(NormGradArgs &a, int dtype, cudaStream_t st);
 
 }  // namespace sph

@@ -29,6 +29,7 @@ NORM_SHAPES = [  # (shape, dim)
     ((1, 1), -1), ((1, 5120), -1), ((3, 7), -1), ((65, 31), -1), ((33, 32), 1), ((5, 33), -1), ((130, 96), -1), ((7, 255), -1),
     ((9, 256), -1), ((4, 257), -1), ((70, 1000), -1), ((17, 1024), -1), ((3, 1025), -1), ((5, 2048), -1), ((11, 4099), -1),
     ((2, 8192), -1), ((3, 8200), -1), ((2, 16384), -1), ((3, 16385), -1), ((2, 40000), -1), ((300, 4096), -1), ((1100, 64), -1),
+    ((1000, 8), -1), ((999, 24), -1), ((515, 72), -1), ((2049, 5), -1), ((777, 13), -1), ((50, 12), -1), ((601, 200), -1), ((2000, 333), -1),
     ((2, 3, 5, 40), -1), ((3, 40, 5), 0), ((100, 1), 1), ((2, 1, 5, 7), 1), ((1, 3, 1, 1), 1), ((2, 5, 3, 11), 1), ((1, 64, 37, 75), 1),
     ((3, 48, 16, 8), 1), ((2, 256, 32, 33), 1), ((2, 255, 8, 8), 1), ((1, 512, 9, 16), 1), ((2, 700, 5, 9), 1), ((1, 1030, 4, 64), 1),
     ((4, 16, 130), 1), ((1, 2, 70000), 1), ((2, 96, 181, 33), 1),
