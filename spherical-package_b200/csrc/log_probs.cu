@@ -373,27 +373,158 @@ template <typename T> __global__ void __launch_bounds__(256) log_probs_many_kern
 }
 
 // ---- planes ----------------------------------------------------------------------------------------------------------
-template <typename T> __global__ void __launch_bounds__(256) log_probs_planes_kernel(LogProbArgs a) {
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+// P neighbouring pixels of a channel: four where planes are aligned for that, else one.
+template <typename T, int P> union PixelVector {
+  T t[P];
+  uint4 q;
+  uint2 d;
+  __device__ __forceinline__ PixelVector() {}
+  __device__ __forceinline__ void load(const T *p) {
+    if constexpr (P == 1) t[0] = *p;
+    else if constexpr (sizeof(T) == 4) q = *(const uint4 *)p;
+    else d = *(const uint2 *)p;
+  }
+  __device__ __forceinline__ void store(T *p) const {
+    if constexpr (P == 1) *p = t[0];
+    else if constexpr (sizeof(T) == 4) *(uint4 *)p = q;
+    else *(uint2 *)p = d;
+  }
+};
+// Numbers of pixels into their image and the rest.
+struct PlaneIndex {
+  FastDiv by;
+  int64_t inner;
+  bool small;
+  static PlaneIndex of(int64_t outer, int64_t inner) {
+    const bool small = outer * inner < ((int64_t)1 << 31);
+    return PlaneIndex{FastDiv::make(small ? (unsigned)inner : 1u), inner, small};
+  }
+  __device__ __forceinline__ int64_t image(int64_t at) const { return small ? (int64_t)by.div((unsigned)at) : at / inner; }
+};
+
+// The K best logits of a pixel so far, the best first; of equal ones the first that came.
+template <int K> struct Best {
+  unsigned order[K];
+  int index[K];
+  __device__ __forceinline__ Best() {
+#pragma unroll
+    for (int i = 0; i < K; i++) order[i] = 0, index[i] = -1;
+  }
+  __device__ __forceinline__ void take(unsigned o, int c) {
+    if (o <= order[K - 1]) return;  // (every order is above 0)
+#pragma unroll
+    for (int i = K - 1; i >= 0; i--) {
+      const bool here = o > order[i], above = i > 0 && o > order[i > 0 ? i - 1 : 0];
+      order[i] = above ? order[i > 0 ? i - 1 : 0] : here ? o : order[i];
+      index[i] = above ? index[i > 0 ? i - 1 : 0] : here ? c : index[i];
+    }
+  }
+};
+
+constexpr int kPlaneChannels = 8;  // read at once
+
+// A thread has P pixels and walks over their channels, eight at a time; with K > 0 it keeps the K best of them on the way.
+template <typename T, int P, int K> __global__ void __launch_bounds__(128) log_probs_planes_kernel(LogProbArgs a, PlaneIndex index) {
+  const int64_t at = ((int64_t)blockIdx.x * 128 + threadIdx.x) * P;
   if (at >= a.outer * a.inner) return;
-  const int64_t o = at / a.inner, i = at % a.inner;
+  const int64_t o = index.image(at), i = at - o * a.inner;
+  const T *x = (const T *)a.x + o * a.C * a.inner + i;
+  Stats st[P];
+  Best<K ? K : 1> best[P];
+  for (int c0 = 0; c0 < a.C; c0 += kPlaneChannels) {
+    PixelVector<T, P> v[kPlaneChannels];
+#pragma unroll
+    for (int c = 0; c < kPlaneChannels; c++) {
+      if (c0 + c < a.C) {
+        v[c].load(x + (c0 + c) * a.inner);
+      } else {
+#pragma unroll
+        for (int p = 0; p < P; p++) v[c].t[p] = from_float<T>(-INFINITY);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < P; p++) {
+      float m = st[p].m;
+#pragma unroll
+      for (int c = 0; c < kPlaneChannels; c++) m = max_nan(m, to_float(v[c].t[p]));
+      st[p].move_to(m);
+      const float base = Stats::base(m);
+#pragma unroll
+      for (int c = 0; c < kPlaneChannels; c++) {
+        const float d = distance(to_float(v[c].t[p]), base), e = exp2_fast(d);
+        st[p].s += e;
+        st[p].t = fmaf(e, d, st[p].t);
+        if (K > 0 && c0 + c < a.C) best[p].take(order_of(to_float(v[c].t[p])), c0 + c);
+      }
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < P; p++) {
+    const int64_t t = a.target[at + p];
+    write_stats(a, at + p, st[p], t, t >= 0 && t < a.C ? to_float(x[t * a.inner + p]) : 0.f);
+#pragma unroll
+    for (int j = 0; j < K; j++)
+      if (j < a.k) {
+        const int64_t to = (o * a.k + j) * a.inner + i + p;
+        a.top_index[to] = best[p].index[j];
+        a.top[to] = st[p].log_prob(value_of(best[p].order[j]));
+      }
+  }
+}
+
+// The best beyond the first eight, eight more in each pass over the channels: those that come after the last.
+template <typename T> __global__ void __launch_bounds__(128) log_probs_planes_more_kernel(LogProbArgs a, PlaneIndex index) {
+  const int64_t at = (int64_t)blockIdx.x * 128 + threadIdx.x;
+  if (at >= a.outer * a.inner) return;
+  const int64_t o = index.image(at), i = at - o * a.inner;
   const T *x = (const T *)a.x + o * a.C * a.inner + i;
   Stats st;
   for (int c = 0; c < a.C; c++) st.add(to_float(x[c * a.inner]));
-  const int64_t t = a.target[at];
-  write_stats(a, at, st, t, t >= 0 && t < a.C ? to_float(x[t * a.inner]) : 0.f);
-  Candidate last = ~0ull;
-  for (int j = 0; j < a.k; j++) {
-    Candidate mine = 0;
+  int64_t to = (o * a.k + 7) * a.inner + i;
+  int last = (int)a.top_index[to];
+  for (int done = 8; done < a.k; done += 8) {
+    const unsigned least = order_of(to_float(x[last * a.inner]));
+    Best<8> best;
     for (int c = 0; c < a.C; c++) {
-      const Candidate q = candidate(order_of(to_float(x[c * a.inner])), c);
-      if (q < last && q > mine) mine = q;
+      const unsigned order = order_of(to_float(x[c * a.inner]));
+      if (order < least || (order == least && c > last)) best.take(order, c);
     }
-    last = mine;
-    const int64_t to = (o * a.k + j) * a.inner + i;
-    a.top_index[to] = candidate_index(mine);
-    a.top[to] = st.log_prob(value_of((unsigned)(mine >> 32)));
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      if (done + j < a.k) {
+        to += a.inner;
+        last = best.index[j];
+        a.top_index[to] = last;
+        a.top[to] = st.log_prob(value_of(best.order[j]));
+      }
   }
+}
+
+template <typename T, int P> void launch_planes(const LogProbArgs &a, cudaStream_t st) {
+  const PlaneIndex index = PlaneIndex::of(a.outer, a.inner);
+  const int64_t threads = a.outer * a.inner / P;
+  const unsigned blocks = (unsigned)((threads + 127) / 128);
+  if (a.k == 0)
+    log_probs_planes_kernel<T, P, 0><<<blocks, 128, 0, st>>>(a, index);
+  else if (a.k == 1)
+    log_probs_planes_kernel<T, P, 1><<<blocks, 128, 0, st>>>(a, index);
+  else if (a.k <= 4)
+    log_probs_planes_kernel<T, P, 4><<<blocks, 128, 0, st>>>(a, index);
+  else
+    log_probs_planes_kernel<T, P, 8><<<blocks, 128, 0, st>>>(a, index);
+}
+template <typename T> bool planes_of_four(int64_t inner, const void *x, const void *gx = nullptr) {
+  return inner % 4 == 0 && ((uintptr_t)x | (uintptr_t)gx) % (4 * sizeof(T)) == 0;
+}
+// Kernels launched.
+template <typename T> int launch_planes(const LogProbArgs &a, cudaStream_t st) {
+  if (planes_of_four<T>(a.inner, a.x) && a.k <= 1)  // (lists of four pixels would not fit the registers)
+    launch_planes<T, 4>(a, st);
+  else
+    launch_planes<T, 1>(a, st);
+  if (a.k <= 8) return 1;
+  log_probs_planes_more_kernel<T><<<(unsigned)((a.outer * a.inner + 127) / 128), 128, 0, st>>>(a, PlaneIndex::of(a.outer, a.inner));
+  return 2;
 }
 
 // ---- gradient --------------------------------------------------------------------------------------------------------
@@ -493,13 +624,52 @@ template <typename T> __global__ void __launch_bounds__(256) log_probs_rows_grad
   }
 }
 
-template <typename T> __global__ void __launch_bounds__(256) log_probs_planes_grad_kernel(LogProbGradArgs a) {
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+// A thread has P pixels, as in the forward pass.
+template <typename T, int P> __global__ void __launch_bounds__(128) log_probs_planes_grad_kernel(LogProbGradArgs a, PlaneIndex index) {
+  const int64_t at = ((int64_t)blockIdx.x * 128 + threadIdx.x) * P;
   if (at >= a.outer * a.inner) return;
-  const int64_t o = at / a.inner, i = at % a.inner, base = o * a.C * a.inner + i;
-  const RowGrad r = row_grad(a, at, o, i);
-  for (int c = 0; c < a.C; c++)
-    ((T *)a.gx)[base + c * a.inner] = from_float<T>(r.of(to_float(((const T *)a.x)[base + c * a.inner])) + own_grad(a, r, o, i, c));
+  const int64_t o = index.image(at), i = at - o * a.inner, base = o * a.C * a.inner + i;
+  const T *x = (const T *)a.x + base;
+  T *gx = (T *)a.gx + base;
+  RowGrad r[P];
+  int target[P];
+#pragma unroll
+  for (int p = 0; p < P; p++) {
+    r[p] = row_grad(a, at + p, o, i + p);
+    target[p] = r[p].target >= 0 && r[p].target < a.C ? (int)r[p].target : -1;
+  }
+  for (int c0 = 0; c0 < a.C; c0 += kPlaneChannels) {
+    PixelVector<T, P> v[kPlaneChannels];
+#pragma unroll
+    for (int c = 0; c < kPlaneChannels; c++)
+      if (c0 + c < a.C) v[c].load(x + (c0 + c) * a.inner);
+#pragma unroll
+    for (int c = 0; c < kPlaneChannels; c++)
+      if (c0 + c < a.C) {
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+          const float d = r[p].of(to_float(v[c].t[p]));
+          v[c].t[p] = from_float<T>(c0 + c == target[p] ? d + r[p].g : d);
+        }
+        v[c].store(gx + (c0 + c) * a.inner);
+      }
+  }
+#pragma unroll
+  for (int p = 0; p < P; p++)  // the most probable classes right behind
+    if (r[p].tops)
+      for (int j = 0; j < a.k; j++) {
+        const int64_t c = a.top_index[(o * a.k + j) * a.inner + i + p];
+        if (c >= 0 && c < a.C)
+          gx[c * a.inner + p] = from_float<T>(r[p].of(to_float(x[c * a.inner + p])) + own_grad(a, r[p], o, i + p, (int)c));
+      }
+}
+template <typename T> void launch_planes_grad(const LogProbGradArgs &a, cudaStream_t st) {
+  const PlaneIndex index = PlaneIndex::of(a.outer, a.inner);
+  const int64_t pixels = a.outer * a.inner;
+  if (planes_of_four<T>(a.inner, a.x, a.gx))
+    log_probs_planes_grad_kernel<T, 4><<<(unsigned)((pixels / 4 + 127) / 128), 128, 0, st>>>(a, index);
+  else
+    log_probs_planes_grad_kernel<T, 1><<<(unsigned)((pixels + 127) / 128), 128, 0, st>>>(a, index);
 }
 
 // Blocks for a row: enough for two on each SM, no more than the row has tiles.
@@ -557,6 +727,7 @@ extern "C" int sph_token_log_probs_forward(const void *x, const int64_t *target,
     return SPH_ERR_INVALID_ARGUMENT;
   const LogProbArgs a{x, target, log_probs, entropy, top, (float2 *)stats, top_index, outer, inner, x_stride, ignore_index, (int)C, (int)k};
   cudaStream_t st = (cudaStream_t)stream;
+  int launches = 1;
   SPH_DISPATCH_ELEMENT(dtype, {
     if (inner == 1 && C <= 1024 - RowVector<T>::N)  // (a row's start may take a part of a vector)
       (k > 0 ? log_probs_warp_kernel<T, true> : log_probs_warp_kernel<T, false>)<<<(unsigned)((outer + 7) / 8), 256, 0, st>>>(a);
@@ -568,9 +739,9 @@ extern "C" int sph_token_log_probs_forward(const void *x, const int64_t *target,
         return SPH_ERR_CUDA;
       }
     } else
-      log_probs_planes_kernel<T><<<(unsigned)((outer * inner + 255) / 256), 256, 0, st>>>(a);
+      launches = launch_planes<T>(a, st);
   });
-  return launch_status();
+  return launch_status(launches);
 }
 
 extern "C" int sph_token_log_probs_backward(const void *x, const int64_t *target, const float *stats, const float *entropy,
@@ -591,7 +762,7 @@ extern "C" int sph_token_log_probs_backward(const void *x, const int64_t *target
     if (inner == 1)
       log_probs_rows_grad_kernel<T><<<row_grid(blocks_per_row(outer, C, 256 * RowVector<T>::N, 64), outer), 256, 0, st>>>(a);
     else
-      log_probs_planes_grad_kernel<T><<<(unsigned)((outer * inner + 255) / 256), 256, 0, st>>>(a);
+      launch_planes_grad<T>(a, st);
   });
   return launch_status();
 }
