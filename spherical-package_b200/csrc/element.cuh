@@ -6,6 +6,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace sph {
@@ -54,6 +56,24 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+// Two float32 operations in one instruction.
+__device__ __forceinline__ unsigned long long as_pair(float2 v) { return __builtin_bit_cast(unsigned long long, v); }
+__device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(as_pair(a)), "l"(as_pair(b)));
+  return __builtin_bit_cast(float2, r);
+}
+__device__ __forceinline__ float2 mul_pair(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(as_pair(a)), "l"(as_pair(b)));
+  return __builtin_bit_cast(float2, r);
+}
+__device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(as_pair(a)), "l"(as_pair(b)), "l"(as_pair(c)));
+  return __builtin_bit_cast(float2, r);
+}
+
 // Sums (or other joins) over the threads of a warp or of a block; every thread gets the same value.
 template <class F> __device__ __forceinline__ float warp_join(float v, F f) {
 #pragma unroll
@@ -90,6 +110,19 @@ __device__ __forceinline__ void copy_4(void *to, const void *from) {
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int PENDING> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
 
+// Two 16-bit elements in a word, the first below.
+template <typename T> struct TwoOf { using Type = __nv_bfloat162; };
+template <> struct TwoOf<__half> { using Type = __half2; };
+template <typename T> __device__ __forceinline__ unsigned two_as_word(float2 v) {
+  typename TwoOf<T>::Type q;
+  if constexpr (std::is_same<T, __half>::value) q = __float22half2_rn(v);
+  else q = __float22bfloat162_rn(v);
+  return *reinterpret_cast<const unsigned *>(&q);
+}
+template <typename T> __device__ __forceinline__ typename TwoOf<T>::Type word_as_two(unsigned w) {
+  return *reinterpret_cast<const typename TwoOf<T>::Type *>(&w);
+}
+
 // 16 bytes of a row at a time.  A row need not start on a 16-byte boundary: vector v holds the elements [v n - shift, v n - shift + n)
 // with `shift` the elements between the boundary before the row and its start; the vectors at its two ends are put together
 // from single elements.
@@ -119,6 +152,33 @@ template <typename T> struct RowVector {
     }
   }
   __device__ __forceinline__ float at(int i) const { return to_float(t[i]); }
+  // An element that is not known at compile time.
+  __device__ __forceinline__ float at_any(int i) const {
+    float v = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; j++) v = i == j ? to_float(t[j]) : v;
+    return v;
+  }
+  __device__ __forceinline__ void set_any(int i, float v) {
+#pragma unroll
+    for (int j = 0; j < N; j++) t[j] = i == j ? from_float<T>(v) : t[j];
+  }
+  // Elements 2 i and 2 i + 1.
+  __device__ __forceinline__ float2 pair(int i) const {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      const unsigned w = i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w;
+      return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    } else {
+      return make_float2(to_float(t[2 * i]), to_float(t[2 * i + 1]));
+    }
+  }
+  __device__ __forceinline__ void set_pair(int i, float2 v) {
+    if constexpr (std::is_same<T, float>::value) {
+      t[2 * i] = v.x, t[2 * i + 1] = v.y;
+    } else {
+      (i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w) = two_as_word<T>(v);
+    }
+  }
 };
 
 // Run a statement with T = the element type of a dtype code.

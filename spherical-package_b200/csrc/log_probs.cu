@@ -38,7 +38,8 @@ __device__ __forceinline__ float exp2_fast(float d) {
 }
 // log2 e times a logit's distance from the maximum; what is infinitely far below stops at a finite distance whose exponential
 // is 0, so that 0 times it is 0.
-__device__ __forceinline__ float distance(float x, float base) { return max_nan((x - base) * kLog2e, -1000.f); }
+constexpr float kFar = -1000.f;
+__device__ __forceinline__ float distance(float x, float base) { return max_nan((x - base) * kLog2e, kFar); }
 
 // Order of the candidates as one number: larger is better; value first (NaN above all), then the lower index.
 __device__ __forceinline__ unsigned order_of(float v) {
@@ -109,9 +110,9 @@ __device__ __forceinline__ void write_stats(const LogProbArgs &a, int64_t at, co
 }
 
 // ---- rows ------------------------------------------------------------------------------------------------------------
-// A thread's part of a tile: 32 logits in registers.
-template <typename T> struct Tile {
-  static constexpr int N = RowVector<T>::N, V = 32 / N;
+// A thread's part of a tile: V vectors of logits in registers.
+template <typename T, int V> struct Tile {
+  static constexpr int N = RowVector<T>::N;
   RowVector<T> v[V];
   // The vectors at, at + step, ... below `end`; the others are -inf.
   __device__ __forceinline__ void load(const T *row, int at, int step, int end, int shift, int C) {
@@ -120,27 +121,42 @@ template <typename T> struct Tile {
     for (int i = 0; i < V; i++) v[i].load(row, at + i * step < end ? (at + i * step) * N - shift : C, C, none);
   }
   __device__ __forceinline__ float largest() const {
-    float m = v[0].at(0);
+    if constexpr (sizeof(T) == 4) {
+      float m = v[0].at(0);
 #pragma unroll
-    for (int i = 0; i < V; i++)
+      for (int i = 0; i < V; i++)
 #pragma unroll
-      for (int j = 0; j < N; j++) m = max_nan(m, v[i].at(j));
-    return m;
+        for (int j = 0; j < N; j++) m = max_nan(m, v[i].at(j));
+      return m;
+    } else {  // two at once
+      auto m = word_as_two<T>(v[0].u.x);
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        m = __hmax2_nan(m, word_as_two<T>(v[i].u.x));
+        m = __hmax2_nan(m, word_as_two<T>(v[i].u.y));
+        m = __hmax2_nan(m, word_as_two<T>(v[i].u.z));
+        m = __hmax2_nan(m, word_as_two<T>(v[i].u.w));
+      }
+      return max_nan(to_float(m.x), to_float(m.y));
+    }
   }
   __device__ __forceinline__ void add_to(Stats &st, float largest) const {
     st.move_to(max_nan(st.m, largest));
     const float base = Stats::base(st.m);
-    float s[2] = {0.f, 0.f}, t[2] = {0.f, 0.f};
+    const float2 off = make_float2(-base, -base), scale = make_float2(kLog2e, kLog2e);
+    float2 s = make_float2(0.f, 0.f), t = s;
 #pragma unroll
     for (int i = 0; i < V; i++)
 #pragma unroll
-      for (int j = 0; j < N; j++) {
-        const float d = distance(v[i].at(j), base), e = exp2_fast(d);
-        s[j & 1] += e;
-        t[j & 1] = fmaf(e, d, t[j & 1]);
+      for (int j = 0; j < N / 2; j++) {
+        float2 d = mul_pair(add_pair(v[i].pair(j), off), scale);
+        d.x = max_nan(d.x, kFar), d.y = max_nan(d.y, kFar);
+        const float2 e = make_float2(exp2_fast(d.x), exp2_fast(d.y));
+        s = add_pair(s, e);
+        t = fma_pair(e, d, t);
       }
-    st.s += s[0] + s[1];
-    st.t += t[0] + t[1];
+    st.s += s.x + s.y;
+    st.t += t.x + t.y;
   }
   // f(order, index) for each logit of order `least` or better.
   template <class F> __device__ __forceinline__ void each(unsigned least, int at, int step, int end, int shift, int C, F f) const {
@@ -165,30 +181,49 @@ __device__ __forceinline__ void rank_candidates(const Candidate *from, int n, in
   }
 }
 
-constexpr int kRowThreads = 256, kRowTile = kRowThreads * 32, kMostTop = 32, kMostCandidates = 1024, kMostCluster = 16;
+// The k-th largest of the lanes' values (k <= 32).
+__device__ __forceinline__ unsigned kth_largest(unsigned v, int k) {
+  unsigned most = 0;
+  for (int i = 0; i < k; i++) {
+    most = __reduce_max_sync(0xffffffffu, v);
+    const unsigned who = __ballot_sync(0xffffffffu, v == most);
+    if ((threadIdx.x & 31) == __ffs(who) - 1) v = 0;
+  }
+  return most;
+}
+
+constexpr int kRowThreads = 256, kMostTop = 32, kMostCandidates = 1024, kMostCluster = 16;
 
 // A row belongs to a cluster of blocks (gridDim.x of them, one where there are rows enough); a block walks its run of vectors in
-// tiles of 8192 logits held in registers, each read once.  Of each tile the best are found without looking at most of it: the k-th
-// largest of the maxima of 32 groups of threads is a bound that k logits reach and few others do.
+// tiles held in registers, each read once, the next one while it works on one.  With TOP (k > 0) it finds the best of each tile
+// without looking at most of it: the k-th largest of the maxima of 32 groups of threads is a bound that k logits reach and few
+// others do.  The blocks of a cluster put what they found into the first one's shared memory.
+template <typename T, bool TOP> struct RowKernel {
+  static constexpr int V = TOP ? 32 / RowVector<T>::N : 4, TILE = kRowThreads * V * RowVector<T>::N;  // logits of a tile
+};
 template <typename T, bool TOP> __global__ void __launch_bounds__(kRowThreads, TOP ? 3 : 4) log_probs_rows_kernel(LogProbArgs a) {
-  __shared__ float4 stats[8], whole;
+  constexpr int V = RowKernel<T, TOP>::V;
+  __shared__ float4 stats[8], parts[kMostCluster], whole;
   __shared__ unsigned group_best[32];
   __shared__ Candidate best[2][kMostTop];
-  __shared__ Candidate pool[TOP ? kMostCandidates : 1];
+  __shared__ Candidate pool[TOP ? kMostCandidates : 1], gathered[TOP ? kMostCluster * kMostTop : 1];
   __shared__ int pooled;
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = (int)gridDim.x, part = (int)blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
   if (row >= a.outer) return;  // (the whole cluster)
+  if (blocks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // I have started
   const T *x = (const T *)a.x + row * a.x_stride;
   const int shift = RowVector<T>::shift_of(x), vectors = (int)(((int64_t)a.C + shift + RowVector<T>::N - 1) / RowVector<T>::N);
   const int per = (vectors + blocks - 1) / blocks, from = min(part * per, vectors), end = min(from + per, vectors);
   Stats st;
   int have = 0, now = 0;  // candidates kept so far, in best[now]
-  for (int v0 = from; v0 < end; v0 += kRowThreads * Tile<T>::V) {
-    Tile<T> tile;
+  Tile<T, V> tile;
+  tile.load(x, from + threadIdx.x, kRowThreads, end, shift, a.C);
+  for (int v0 = from; v0 < end; v0 += kRowThreads * V) {
     const int at = v0 + threadIdx.x;
-    tile.load(x, at, kRowThreads, end, shift, a.C);
+    Tile<T, V> next;
+    if (!TOP && v0 + kRowThreads * V < end) next.load(x, at + kRowThreads * V, kRowThreads, end, shift, a.C);
     const float largest = tile.largest();
     if (TOP) {
       const unsigned mine = order_of(largest);
@@ -199,15 +234,8 @@ template <typename T, bool TOP> __global__ void __launch_bounds__(kRowThreads, T
       if (threadIdx.x < have) pool[threadIdx.x] = best[now][threadIdx.x];
       if (threadIdx.x == 0) pooled = have;
       __syncthreads();
-      o = group_best[lane];
-      unsigned least = 0;
-      for (int i = 0; i < a.k; i++) {  // the k-th largest of the groups' best
-        least = __reduce_max_sync(0xffffffffu, o);
-        const unsigned who = __ballot_sync(0xffffffffu, o == least);
-        if (lane == __ffs(who) - 1) o = 0;
-      }
       const Candidate worst = have == a.k ? best[now][a.k - 1] : 0;
-      least = max(least, (unsigned)(worst >> 32));
+      const unsigned least = max(kth_largest(group_best[lane], a.k), (unsigned)(worst >> 32));
       if (mine >= least)
         tile.each(least, at, kRowThreads, end, shift, a.C, [&](unsigned order, int index) {
           const Candidate c = candidate(order, index);
@@ -249,72 +277,97 @@ template <typename T, bool TOP> __global__ void __launch_bounds__(kRowThreads, T
       __syncthreads();
     }
     tile.add_to(st, largest);
+    if (TOP) {
+      if (v0 + kRowThreads * V < end) tile.load(x, at + kRowThreads * V, kRowThreads, end, shift, a.C);
+    } else {
+      tile = next;
+    }
   }
   st.join_warp();
   if (lane == 0) stats[warp] = st.packed();
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < 8; i++) st.join(Stats::of(stats[i]));
-    whole = st.packed();
-    pooled = have;
-    if (TOP && now == 1)
-      for (int i = 0; i < have; i++) best[0][i] = best[1][i];
-  }
-  if (blocks == 1) {
-    __syncthreads();
-  } else {
-    cluster.sync();
-    if (part == 0) {
-      // a thread per candidate of the others' lists; the first thread of all joins the statistics
-      if (TOP) {
-        int n = 0;
-        for (int b = 0; b < blocks; b++) {
-          const int more = *cluster.map_shared_rank(&pooled, b);
-          for (int i = threadIdx.x; i < more; i += kRowThreads) pool[n + i] = cluster.map_shared_rank(&best[0][0], b)[i];
-          n += more;
-        }
-        __syncthreads();
-        rank_candidates(pool, n, a.k, best[1]);
-      }
-      if (threadIdx.x == 0) {
-        for (int b = 1; b < blocks; b++) st.join(Stats::of(*cluster.map_shared_rank(&whole, b)));
-        whole = st.packed();
-      }
-      __syncthreads();
+  if (blocks > 1) {
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every block has started, so its shared memory may be written
+    if (threadIdx.x == 0) {
+      for (int i = 1; i < 8; i++) st.join(Stats::of(stats[i]));
+      cluster.map_shared_rank(&parts[0], 0)[part] = st.packed();
     }
-    cluster.sync();  // what was read of the others has to last until here
+    if (TOP && threadIdx.x < a.k)
+      cluster.map_shared_rank(&gathered[0], 0)[part * a.k + threadIdx.x] = threadIdx.x < have ? best[now][threadIdx.x] : 0;
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (part != 0) return;
-    now = 1;
+    if (TOP) {
+      rank_candidates(gathered, blocks * a.k, a.k, best[now ^ 1]);
+      now ^= 1;
+    }
   }
   if (threadIdx.x == 0) {
+    const int n = blocks > 1 ? blocks : 8;
+    const float4 *all = blocks > 1 ? parts : stats;
+    st = Stats::of(all[0]);
+    for (int i = 1; i < n; i++) st.join(Stats::of(all[i]));
+    whole = st.packed();
     const int64_t t = a.target[row];
-    write_stats(a, row, Stats::of(whole), t, t >= 0 && t < a.C ? to_float(x[t]) : 0.f);
+    write_stats(a, row, st, t, t >= 0 && t < a.C ? to_float(x[t]) : 0.f);
   }
-  if (TOP && threadIdx.x < a.k) {
-    const Candidate c = best[blocks == 1 ? 0 : 1][threadIdx.x];
+  if (!TOP) return;
+  __syncthreads();
+  if (threadIdx.x < a.k) {
+    const Candidate c = best[now][threadIdx.x];
     a.top_index[row * a.k + threadIdx.x] = candidate_index(c);
     a.top[row * a.k + threadIdx.x] = Stats::of(whole).log_prob(value_of((unsigned)(c >> 32)));
   }
 }
 
-// Rows of up to 1024 classes: a warp each, their logits in registers.
+// Rows of up to 1024 classes: a warp each, their logits in registers; the best by the same bound, of the maxima of the lanes.
 template <typename T, bool TOP> __global__ void __launch_bounds__(256, TOP ? 2 : 4) log_probs_warp_kernel(LogProbArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  constexpr int V = 32 / RowVector<T>::N, POOL = 96;
+  __shared__ Candidate pools[TOP ? 8 : 1][POOL];
+  __shared__ int counts[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * 8 + warp;
   if (row >= a.outer) return;
   const T *x = (const T *)a.x + row * a.x_stride;
   const int shift = RowVector<T>::shift_of(x), vectors = (a.C + shift + RowVector<T>::N - 1) / RowVector<T>::N;
-  Tile<T> tile;
+  Tile<T, V> tile;
   tile.load(x, lane, 32, vectors, shift, a.C);
   const int64_t t = a.target[row];
-  const float x_t = t >= 0 && t < a.C ? to_float(x[t]) : 0.f;
+  const float x_t = t >= 0 && t < a.C ? to_float(x[t]) : 0.f, largest = tile.largest();
   Stats st;
-  tile.add_to(st, tile.largest());
+  tile.add_to(st, largest);
   st.join_warp();
   if (lane == 0) write_stats(a, row, st, t, x_t);
   if (!TOP) return;
-  Candidate last = ~0ull;
-  for (int i = 0; i < a.k; i++) {  // the best below the last
+  const auto put = [&](int i, Candidate c) {
+    a.top_index[row * a.k + i] = candidate_index(c);
+    a.top[row * a.k + i] = st.log_prob(value_of((unsigned)(c >> 32)));
+  };
+  Candidate *pool = pools[TOP ? warp : 0];
+  int n = POOL + 1;
+  if (a.k <= 32) {
+    const unsigned mine = order_of(largest), least = kth_largest(mine, a.k);
+    if (lane == 0) counts[warp] = 0;
+    __syncwarp();
+    if (mine >= least)
+      tile.each(least, lane, 32, vectors, shift, a.C, [&](unsigned order, int index) {
+        const int to = atomicAdd(&counts[warp], 1);
+        if (to < POOL) pool[to] = candidate(order, index);
+      });
+    __syncwarp();
+    n = counts[warp];
+  }
+  if (n <= POOL) {
+    for (int i = lane; i < n; i += 32) {
+      const Candidate c = pool[i];
+      int rank = 0;
+      for (int j = 0; j < n; j++) rank += pool[j] > c;
+      if (rank < a.k) put(rank, c);
+    }
+    return;
+  }
+  Candidate last = ~0ull;  // very many alike, or wanted: each the best below the last
+  for (int i = 0; i < a.k; i++) {
     Candidate c = 0;
     tile.each(0, lane, 32, vectors, shift, a.C, [&](unsigned order, int index) {
       const Candidate q = candidate(order, index);
@@ -323,10 +376,7 @@ template <typename T, bool TOP> __global__ void __launch_bounds__(256, TOP ? 2 :
     const unsigned order = __reduce_max_sync(0xffffffffu, (unsigned)(c >> 32));
     const unsigned index = __reduce_max_sync(0xffffffffu, (unsigned)(c >> 32) == order ? (unsigned)c : 0u);
     last = (Candidate)order << 32 | index;
-    if (lane == 0) {
-      a.top_index[row * a.k + i] = candidate_index(last);
-      a.top[row * a.k + i] = st.log_prob(value_of(order));
-    }
+    if (lane == 0) put(i, last);
   }
 }
 
@@ -548,6 +598,11 @@ struct RowGrad {
     const float d = distance(x, m);
     return exp2_fast(d) * fmaf(slope, d, flat);
   }
+  __device__ __forceinline__ float2 of(float2 x) const {
+    float2 d = mul_pair(add_pair(x, make_float2(-m, -m)), make_float2(kLog2e, kLog2e));
+    d.x = max_nan(d.x, kFar), d.y = max_nan(d.y, kFar);
+    return mul_pair(make_float2(exp2_fast(d.x), exp2_fast(d.y)), fma_pair(make_float2(slope, slope), d, make_float2(flat, flat)));
+  }
 };
 // `at`: the distribution's number, `o`, `i`: its parts.
 __device__ __forceinline__ RowGrad row_grad(const LogProbGradArgs &a, int64_t at, int64_t o, int64_t i) {
@@ -606,11 +661,11 @@ template <typename T> __global__ void __launch_bounds__(256) log_probs_rows_grad
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const int at = v0 + i * 256 + threadIdx.x, first = at < end ? at * N - shift : a.C;
+      const bool here = target >= first && target < first + N;
+      const float g_t = here ? r.of(v[i].at_any(target - first)) + r.g : 0.f;
 #pragma unroll
-      for (int j = 0; j < N; j++) {
-        const float d = r.of(v[i].at(j));
-        v[i].t[j] = from_float<T>(first + j == target ? d + r.g : d);
-      }
+      for (int j = 0; j < N / 2; j++) v[i].set_pair(j, r.of(v[i].pair(j)));
+      if (here) v[i].set_any(target - first, g_t);
       v[i].store(gx, first, a.C);
     }
   }
@@ -686,7 +741,7 @@ inline dim3 row_grid(int n, int64_t rows) {
 }
 
 template <typename T> cudaError_t launch_rows(const LogProbArgs &a, cudaStream_t st) {
-  const int n = blocks_per_row(a.outer, a.C, kRowTile, kMostCluster);
+  const int n = blocks_per_row(a.outer, a.C, a.k > 0 ? RowKernel<T, true>::TILE : RowKernel<T, false>::TILE, kMostCluster);
   void (*kernel)(LogProbArgs) = a.k > 0 ? log_probs_rows_kernel<T, true> : log_probs_rows_kernel<T, false>;
   cudaLaunchConfig_t config = {};
   config.gridDim = row_grid(n, a.outer);
