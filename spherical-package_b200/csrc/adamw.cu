@@ -10,6 +10,8 @@
 // What is not finite is held as NaN, and leaves the other values of its 256 as they are.
 #include "element.cuh"
 
+#include <algorithm>
+
 namespace sph {
 
 constexpr int kAdamBlock = 256;  // values behind one scale, and what a warp takes at once: eight a lane
@@ -77,10 +79,47 @@ __device__ __forceinline__ void store8(E4m3 *p, const float (&v)[8]) {
   *(uint2 *)p = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
 }
 
+// A lane's eight values as they are in memory.
+template <typename T> struct Raw {
+  unsigned w[2 * sizeof(T)];
+  __device__ __forceinline__ void load(const T *p) {
+    if constexpr (sizeof(T) == 4) {
+      asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                   : "l"(p));
+    } else if constexpr (sizeof(T) == 2) {
+      const uint4 q = *(const uint4 *)p;
+      w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+    } else {
+      const uint2 q = *(const uint2 *)p;
+      w[0] = q.x, w[1] = q.y;
+    }
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if constexpr (sizeof(T) == 4) {
+        v[2 * i] = __uint_as_float(w[2 * i]), v[2 * i + 1] = __uint_as_float(w[2 * i + 1]);
+      } else if constexpr (sizeof(T) == 1) {
+        const unsigned two = (w[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+        const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3)));
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+      } else if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(word_as_two<T>(w[i]));
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+      } else {
+        v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
+  }
+};
+
 // A lane's eight of a warp's 256 values: neighbours, or every 32nd where the tensor is not aligned for that or ends inside.
 template <typename T> __device__ __forceinline__ void load_lane(const T *p, int lane, bool wide, int n, float (&v)[8]) {
   if (wide) {
-    load8(p + 8 * lane, v);
+    Raw<T> q;
+    q.load(p + 8 * lane);
+    q.values(v);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] = lane + 32 * i < n ? to_float(p[lane + 32 * i]) : 0.f;
@@ -96,13 +135,14 @@ template <typename T> __device__ __forceinline__ void store_lane(T *p, int lane,
   }
 }
 
-// Codes and scale of a warp's 256 values.
-__device__ __forceinline__ float encode(float (&v)[8], bool root) {
+// Largest magnitude of a warp's 256 values; NaN is passed over, and its code is NaN; infinities become NaN and leave the others
+// alone.
+__device__ __forceinline__ float largest_of(float (&v)[8]) {
   float amax = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(v[i]));  // (NaN is passed over, and its code is NaN)
+  for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(v[i]));
   amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
-  if (amax == INFINITY) {  // infinities become NaN and leave the others alone
+  if (amax == INFINITY) {
     amax = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
@@ -111,18 +151,26 @@ __device__ __forceinline__ float encode(float (&v)[8], bool root) {
     }
     amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
   }
-  const Scale s = Scale::of(amax);
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    v[i] *= s.inverse;
-    if (root) v[i] = v[i] > 0.f ? fmaxf(v[i], 0x1p-9f) : v[i];
-  }
-  return s.scale;
+  return amax;
 }
+// Two scales at once: amax / 448 and 448 / amax of both are one division, in four lanes of four.
+struct Scales {
+  float m, m_inverse, u, u_inverse;
+  __device__ __forceinline__ Scales(float m_max, float u_max) {
+    const int lane = threadIdx.x & 31;
+    const float amax = lane & 2 ? u_max : m_max;
+    const float q = amax < kTiny ? 0.f : (lane & 1 ? kE4m3Max : amax) / (lane & 1 ? amax : kE4m3Max);
+    m = __shfl_sync(0xffffffffu, q, 0), m_inverse = __shfl_sync(0xffffffffu, q, 1);
+    u = __shfl_sync(0xffffffffu, q, 2), u_inverse = __shfl_sync(0xffffffffu, q, 3);
+  }
+};
 
-// A warp takes up to `chunk` blocks of 256 values of one tensor.
+// A warp takes up to `chunk` blocks of 256 values of one tensor.  With 8-bit moments, of which fewer bytes are on their way for the
+// same work, it fetches the next block while it works on one (332M bf16 weights with masters: 1146 us without, 875 with; through
+// asynchronous copies into shared memory, which leave less L1 for what plain loads have on their way, 983).
 template <typename P, typename G, bool EIGHT, bool MASTER, int CAP>
-__global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ AdamArgs<CAP> a) {
+__global__ void __launch_bounds__(256, EIGHT ? 3 : 4) adamw_kernel(const __grid_constant__ AdamArgs<CAP> a) {
+  using W = typename std::conditional<MASTER, float, P>::type;  // what is updated
   const int lane = threadIdx.x & 31, task = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (task >= a.first[a.tensors]) return;
   int lo = 0, hi = a.tensors;  // the tensor that holds the task: first[lo] <= task < first[hi]
@@ -132,7 +180,24 @@ __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Adam
   }
   const AdamTensor &t = a.tensor[lo];
   const bool aligned = a.aligned[lo];
+  const W *weights = MASTER ? (const W *)t.master : (const W *)t.param;
+  int64_t b = (int64_t)(task - a.first[lo]) * a.chunk;
+  const int count = (int)min((int64_t)a.chunk, (t.n + kAdamBlock - 1) / kAdamBlock - b);
+  Raw<W> w_next;
+  Raw<G> g_next;
+  Raw<E4m3> m_next, v_next;
   float lr = a.lr, step_size = a.step_size, root = a.root;
+  const auto fetch = [&](int j) {  // the j-th block from here on
+    const int64_t at = (b + j) * kAdamBlock;
+    if (j >= count) return;
+    if (aligned && at + kAdamBlock <= t.n) {
+      w_next.load(weights + at + 8 * lane);
+      g_next.load((const G *)t.grad + at + 8 * lane);
+      m_next.load((const E4m3 *)t.m + at + 8 * lane);
+      v_next.load((const E4m3 *)t.v + at + 8 * lane);
+    }
+  };
+  if (EIGHT) fetch(0);
   if (a.step_at) {
     if (a.lr_at) lr = *a.lr_at;
     const double step = (double)*a.step_at;
@@ -140,51 +205,66 @@ __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Adam
     root = (float)(1.0 / sqrt(-expm1(step * a.log_beta2)));
   }
   const float keep = 1.f - lr * a.decay;
-  int64_t b = (int64_t)(task - a.first[lo]) * a.chunk;
-  for (int j = 0; j < a.chunk; j++, b++) {
-    const int64_t at = b * kAdamBlock;
-    if (at >= t.n) return;
+  for (int j = 0; j < count; j++) {
+    const int64_t at = (b + j) * kAdamBlock;
     const int n = t.n - at < kAdamBlock ? (int)(t.n - at) : kAdamBlock;
     const bool wide = n == kAdamBlock && aligned;
-    float w[8], g[8], m[8], v[8], u[8];
-    load_lane((const G *)t.grad + at, lane, wide, n, g);
-    if (MASTER)
-      load_lane(t.master + at, lane, wide, n, w);
-    else
-      load_lane((const P *)t.param + at, lane, wide, n, w);
-    if (EIGHT) {
-      load_lane((const E4m3 *)t.m + at, lane, wide, n, m);
-      load_lane((const E4m3 *)t.v + at, lane, wide, n, v);
-      const float ms = t.m_scale[b], vs = t.v_scale[b];
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        m[i] *= ms;
-        v[i] *= vs;
-        v[i] *= v[i];
-      }
+    float w[8], g[8], m[8], v[8];
+    const float ms = EIGHT ? t.m_scale[b + j] : 0.f, vs = EIGHT ? t.v_scale[b + j] : 0.f;
+    if (EIGHT && wide) {
+      w_next.values(w);
+      g_next.values(g);
+      m_next.values(m);
+      v_next.values(v);
     } else {
-      load_lane((const float *)t.m + at, lane, wide, n, m);
-      load_lane((const float *)t.v + at, lane, wide, n, v);
+      load_lane(weights + at, lane, wide, n, w);
+      load_lane((const G *)t.grad + at, lane, wide, n, g);
+      if (EIGHT) {
+        load_lane((const E4m3 *)t.m + at, lane, wide, n, m);
+        load_lane((const E4m3 *)t.v + at, lane, wide, n, v);
+      } else {
+        load_lane((const float *)t.m + at, lane, wide, n, m);
+        load_lane((const float *)t.v + at, lane, wide, n, v);
+      }
     }
+    if (EIGHT) fetch(j + 1);
     // The old moment's product and the root are rounded by themselves, the new term is fused: codes are cut from these
     // values, and would otherwise depend on what the compiler fuses.
+    const auto two = [](float x) { return make_float2(x, x); };
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const float gi = g[i] * a.grad_scale;
-      m[i] = fmaf(a.rest1, gi, __fmul_rn(a.beta1, m[i]));
-      v[i] = fmaf(__fmul_rn(a.rest2, gi), gi, __fmul_rn(a.beta2, v[i]));
-      u[i] = sqrtf(v[i]);
-      w[i] = fmaf(-step_size, __fdividef(m[i], fmaf(u[i], root, a.eps)), w[i] * keep);
+    for (int i = 0; i < 8; i += 2) {
+      float2 gi = make_float2(g[i], g[i + 1]), mi = make_float2(m[i], m[i + 1]), vi = make_float2(v[i], v[i + 1]), wi = make_float2(w[i], w[i + 1]);
+      if (EIGHT) {
+        mi = mul_pair(mi, two(ms));
+        vi = mul_pair(vi, two(vs));
+        vi = mul_pair(vi, vi);
+      }
+      gi = mul_pair(gi, two(a.grad_scale));
+      mi = fma_pair(two(a.rest1), gi, mul_pair(two(a.beta1), mi));
+      vi = fma_pair(mul_pair(two(a.rest2), gi), gi, mul_pair(two(a.beta2), vi));
+      const float2 u = make_float2(sqrtf(vi.x), sqrtf(vi.y)), d = fma_pair(u, two(root), two(a.eps));
+      const float2 q = make_float2(__fdividef(mi.x, d.x), __fdividef(mi.y, d.y));
+      wi = fma_pair(two(-step_size), q, mul_pair(wi, two(keep)));
+      w[i] = wi.x, w[i + 1] = wi.y, m[i] = mi.x, m[i + 1] = mi.y;
+      v[i] = EIGHT ? u.x : vi.x, v[i + 1] = EIGHT ? u.y : vi.y;
     }
     if (MASTER) store_lane(t.master + at, lane, wide, n, w);
     store_lane((P *)t.param + at, lane, wide, n, w);
     if (EIGHT) {
-      const float ms = encode(m, false), us = encode(u, true);
+      const float m_max = largest_of(m), u_max = largest_of(v);
+      const Scales scale(m_max, u_max);
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const float2 p = mul_pair(make_float2(m[i], m[i + 1]), two(scale.m_inverse)), q = mul_pair(make_float2(v[i], v[i + 1]), two(scale.u_inverse));
+        m[i] = p.x, m[i + 1] = p.y;
+        v[i] = q.x > 0.f ? fmaxf(q.x, 0x1p-9f) : q.x;
+        v[i + 1] = q.y > 0.f ? fmaxf(q.y, 0x1p-9f) : q.y;
+      }
       store_lane((E4m3 *)t.m + at, lane, wide, n, m);
-      store_lane((E4m3 *)t.v + at, lane, wide, n, u);
+      store_lane((E4m3 *)t.v + at, lane, wide, n, v);
       if (lane == 0) {
-        t.m_scale[b] = ms;
-        t.v_scale[b] = us;
+        t.m_scale[b + j] = scale.m;
+        t.v_scale[b + j] = scale.u;
       }
     } else {
       store_lane((float *)t.m + at, lane, wide, n, m);
@@ -192,7 +272,6 @@ __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Adam
     }
   }
 }
-
 inline bool wide_aligned(const AdamTensor &t, int param_size, int grad_size, int state_size) {
   return ((uintptr_t)t.param % (8 * param_size) | (uintptr_t)t.grad % (8 * grad_size) | (uintptr_t)t.m % (8 * state_size) |
           (uintptr_t)t.v % (8 * state_size) | (uintptr_t)t.master % 32) == 0;
@@ -245,8 +324,9 @@ static int adamw_group(int from, int count, void *const *params, const void *con
   a.step_size = common.step_size, a.root = common.root, a.lr_at = common.lr_at, a.step_at = common.step_at;
   int64_t blocks = 0;
   for (int i = 0; i < count; i++) blocks += (numels[from + i] + kAdamBlock - 1) / kAdamBlock;
-  // A warp finds its tensor once for four blocks, where there are enough of those for every SM's 64 warps twice over.
-  a.chunk = blocks >= 148 * 64 * 8 ? 4 : 1;
+  // A warp finds its tensor once for up to 32 blocks (4 of 32-bit moments, which are as fast one by one and faster side by side:
+  // 174M float32 weights 719 us in fours, 743 in 32s), as long as every SM's 64 warps have two such tasks.
+  a.chunk = (int)std::min<int64_t>(state_bits == 8 ? 32 : 4, std::max<int64_t>(1, blocks / (148 * 64 * 2)));
   int64_t tasks = 0;
   for (int i = 0; i < count; i++) {
     const int k = from + i;

@@ -104,6 +104,9 @@ template <class F> __device__ __forceinline__ float block_join(float v, float *s
 __device__ __forceinline__ void copy_16(void *to, const void *from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
 }
+__device__ __forceinline__ void copy_8(void *to, const void *from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
 __device__ __forceinline__ void copy_4(void *to, const void *from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
 }

@@ -14,6 +14,8 @@
 
 #include <cooperative_groups.h>
 
+#include <algorithm>
+
 namespace sph {
 
 namespace cg = cooperative_groups;
@@ -116,9 +118,15 @@ template <typename T, int V> struct Tile {
   RowVector<T> v[V];
   // The vectors at, at + step, ... below `end`; the others are -inf.
   __device__ __forceinline__ void load(const T *row, int at, int step, int end, int shift, int C) {
-    const T none = from_float<T>(-INFINITY);
+    const T *p = row + ((int64_t)at * N - shift);
+    if (at * N >= shift && at + (V - 1) * step < end && (at + (V - 1) * step) * N - shift + N <= C) {
 #pragma unroll
-    for (int i = 0; i < V; i++) v[i].load(row, at + i * step < end ? (at + i * step) * N - shift : C, C, none);
+      for (int i = 0; i < V; i++) v[i].u = *(const uint4 *)(p + i * step * N);
+    } else {
+      const T none = from_float<T>(-INFINITY);
+#pragma unroll
+      for (int i = 0; i < V; i++) v[i].load(row, at + i * step < end ? (at + i * step) * N - shift : C, C, none);
+    }
   }
   __device__ __forceinline__ float largest() const {
     if constexpr (sizeof(T) == 4) {
@@ -220,12 +228,20 @@ template <typename T, bool TOP> __global__ void __launch_bounds__(kRowThreads, T
   int have = 0, now = 0;  // candidates kept so far, in best[now]
   Tile<T, V> tile;
   tile.load(x, from + threadIdx.x, kRowThreads, end, shift, a.C);
-  for (int v0 = from; v0 < end; v0 += kRowThreads * V) {
+  constexpr int STEP = kRowThreads * V;
+  if (!TOP) {
+    for (int v0 = from; v0 < end; v0 += 2 * STEP) {
+      Tile<T, V> next;
+      next.load(x, v0 + STEP + threadIdx.x, kRowThreads, end, shift, a.C);
+      tile.add_to(st, tile.largest());
+      tile.load(x, v0 + 2 * STEP + threadIdx.x, kRowThreads, end, shift, a.C);
+      next.add_to(st, next.largest());
+    }
+  }
+  for (int v0 = from; TOP && v0 < end; v0 += STEP) {
     const int at = v0 + threadIdx.x;
-    Tile<T, V> next;
-    if (!TOP && v0 + kRowThreads * V < end) next.load(x, at + kRowThreads * V, kRowThreads, end, shift, a.C);
     const float largest = tile.largest();
-    if (TOP) {
+    {
       const unsigned mine = order_of(largest);
       unsigned o = mine;
 #pragma unroll
@@ -277,11 +293,7 @@ template <typename T, bool TOP> __global__ void __launch_bounds__(kRowThreads, T
       __syncthreads();
     }
     tile.add_to(st, largest);
-    if (TOP) {
-      if (v0 + kRowThreads * V < end) tile.load(x, at + kRowThreads * V, kRowThreads, end, shift, a.C);
-    } else {
-      tile = next;
-    }
+    if (v0 + STEP < end) tile.load(x, at + STEP, kRowThreads, end, shift, a.C);
   }
   st.join_warp();
   if (lane == 0) stats[warp] = st.packed();
@@ -317,6 +329,84 @@ template <typename T, bool TOP> __global__ void __launch_bounds__(kRowThreads, T
     const Candidate c = best[now][threadIdx.x];
     a.top_index[row * a.k + threadIdx.x] = candidate_index(c);
     a.top[row * a.k + threadIdx.x] = Stats::of(whole).log_prob(value_of((unsigned)(c >> 32)));
+  }
+}
+
+// Many rows without best classes: the blocks walk over the rows, and their next tiles, of the next rows too, are on their way into
+// shared memory, where every thread reads what it has copied itself.
+constexpr int kRowStages = 3, kStreamThreads = 128, kStreamBlocks = 8;
+template <typename T> __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) log_probs_stream_kernel(LogProbArgs a) {
+  constexpr int V = 4, N = RowVector<T>::N, STEP = kStreamThreads * V;
+  extern __shared__ __align__(16) unsigned char row_memory[];
+  __shared__ float4 stats[2][kStreamThreads / 32];
+  RowVector<T> *slots = (RowVector<T> *)row_memory + threadIdx.x;  // (stage, vector) x threads
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const T none = from_float<T>(-INFINITY);
+  struct Place {  // a tile
+    int64_t row;
+    int v0, shift, vectors;
+    const T *x;
+    __device__ __forceinline__ void open(const LogProbArgs &a, int64_t r) {
+      row = r, v0 = 0;
+      x = (const T *)a.x + r * a.x_stride;
+      shift = RowVector<T>::shift_of(x);
+      vectors = (int)(((int64_t)a.C + shift + N - 1) / N);
+    }
+    __device__ __forceinline__ void next(const LogProbArgs &a) {
+      v0 += STEP;
+      if (v0 >= vectors) open(a, row + gridDim.x);
+    }
+  };
+  Place ahead, here;
+  ahead.open(a, blockIdx.x);
+  here = ahead;
+  const auto copy = [&](int stage) {
+    if (ahead.row < a.outer) {
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        const int at = ahead.v0 + i * kStreamThreads + threadIdx.x, first = at * N - ahead.shift;
+        RowVector<T> *to = slots + (stage * V + i) * kStreamThreads;
+        if (first >= 0 && first + N <= a.C)
+          copy_16(to, ahead.x + first);
+        else if (at < ahead.vectors)
+          for (int j = 0; j < N; j++) to->t[j] = first + j >= 0 && first + j < a.C ? ahead.x[first + j] : none;
+      }
+      ahead.next(a);
+    }
+    copies_end();
+  };
+  for (int d = 0; d < kRowStages - 1; d++) copy(d);
+  Stats st;
+  int stage = 0, turn = 0;
+  while (here.row < a.outer) {
+    copy(stage == 0 ? kRowStages - 1 : stage - 1);
+    copies_wait<kRowStages - 1>();
+    Tile<T, V> tile;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      if (here.v0 + i * kStreamThreads + (int)threadIdx.x < here.vectors) {
+        tile.v[i].u = slots[(stage * V + i) * kStreamThreads].u;
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; j++) tile.v[i].t[j] = none;
+      }
+    }
+    tile.add_to(st, tile.largest());
+    stage = stage == kRowStages - 1 ? 0 : stage + 1;
+    const int64_t row = here.row;
+    const T *x = here.x;
+    here.next(a);
+    if (here.row == row) continue;
+    st.join_warp();
+    if (lane == 0) stats[turn][warp] = st.packed();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int i = 1; i < kStreamThreads / 32; i++) st.join(Stats::of(stats[turn][i]));
+      const int64_t t = a.target[row];
+      write_stats(a, row, st, t, t >= 0 && t < a.C ? to_float(x[t]) : 0.f);
+    }
+    st = Stats();
+    turn ^= 1;
   }
 }
 
@@ -742,6 +832,12 @@ inline dim3 row_grid(int n, int64_t rows) {
 
 template <typename T> cudaError_t launch_rows(const LogProbArgs &a, cudaStream_t st) {
   const int n = blocks_per_row(a.outer, a.C, a.k > 0 ? RowKernel<T, true>::TILE : RowKernel<T, false>::TILE, kMostCluster);
+  if (a.k == 0 && n == 1) {
+    constexpr int bytes = kRowStages * 4 * kStreamThreads * 16;
+    static_assert(bytes <= 32768, "more needs an attribute of the kernel");
+    log_probs_stream_kernel<T><<<(unsigned)std::min<int64_t>(a.outer, 148 * kStreamBlocks), kStreamThreads, bytes, st>>>(a);
+    return cudaGetLastError();
+  }
   void (*kernel)(LogProbArgs) = a.k > 0 ? log_probs_rows_kernel<T, true> : log_probs_rows_kernel<T, false>;
   cudaLaunchConfig_t config = {};
   config.gridDim = row_grid(n, a.outer);

@@ -20,6 +20,7 @@
 
 namespace {
 
+namespace py = pybind11;
 using torch::Tensor;
 using torch::autograd::Node;
 using torch::autograd::SavedVariable;
@@ -353,24 +354,51 @@ c10::optional<std::vector<Tensor>> token_log_probs(const Tensor &x, const Tensor
 }
 
 // ---- AdamW -----------------------------------------------------------------------------------------------------------
-using Tensors = std::vector<Tensor>;
-using OptTensors = c10::optional<std::vector<OptTensor>>;
+// A Python list or tuple of tensors, or None for no list; read where it is (a network's parameters make hundreds of tensors a
+// step, and copying them would take longer than the step).  The caller holds the list and the interpreter's lock.
+class TensorList {
+ public:
+  TensorList(const py::object &o, const char *name) : name_(name) {
+    if (o.is_none()) return;
+    seq_ = py::reinterpret_steal<py::object>(PySequence_Fast(o.ptr(), "adamw_step takes lists of tensors"));
+    if (!seq_) throw py::error_already_set();
+    items_ = PySequence_Fast_ITEMS(seq_.ptr());
+    size_ = (size_t)PySequence_Fast_GET_SIZE(seq_.ptr());
+  }
+  explicit operator bool() const { return items_ != nullptr || seq_; }
+  size_t size() const { return size_; }
+  bool has(size_t i) const { return items_[i] != Py_None; }
+  const Tensor &operator[](size_t i) const {
+    TORCH_CHECK_TYPE(THPVariable_Check(items_[i]), "adamw_step: every ", name_, " must be a tensor");
+    return THPVariable_Unpack(items_[i]);
+  }
 
-void adamw_step(const Tensors &params, const Tensors &grads, const Tensors &m, const Tensors &v, const OptTensors &masters,
-                const c10::optional<Tensors> &m_scales, const c10::optional<Tensors> &v_scales, double step, double lr, double beta1,
-                double beta2, double eps, double weight_decay, double grad_scale, const OptTensor &step_at, const OptTensor &lr_at) {
+ private:
+  const char *name_;
+  py::object seq_;
+  PyObject **items_ = nullptr;
+  size_t size_ = 0;
+};
+
+void adamw_step(const py::object &params_list, const py::object &grads_list, const py::object &m_list, const py::object &v_list,
+                const py::object &masters_list, const py::object &m_scales_list, const py::object &v_scales_list, double step, double lr,
+                double beta1, double beta2, double eps, double weight_decay, double grad_scale, const OptTensor &step_at,
+                const OptTensor &lr_at) {
+  const TensorList params(params_list, "param"), grads(grads_list, "grad"), m(m_list, "exp_avg"), v(v_list, "exp_avg_sq"),
+      masters(masters_list, "master"), m_scales(m_scales_list, "exp_avg_scale"), v_scales(v_scales_list, "exp_avg_sq_scale");
   const size_t n = params.size();
-  TORCH_CHECK(grads.size() == n && m.size() == n && v.size() == n && (!masters || masters->size() == n) &&
-                  (!m_scales || m_scales->size() == n) && (!v_scales || v_scales->size() == n),
+  TORCH_CHECK(grads.size() == n && m.size() == n && v.size() == n && (!masters || masters.size() == n) && (!m_scales || m_scales.size() == n) &&
+                  (!v_scales || v_scales.size() == n),
               "adamw_step: the lists must have the same length");
-  TORCH_CHECK(m_scales.has_value() == v_scales.has_value(), "adamw_step: both moments have scales, or neither");
+  TORCH_CHECK((bool)m_scales == (bool)v_scales, "adamw_step: both moments have scales, or neither");
   TORCH_CHECK(lr >= 0 && std::isfinite(lr) && weight_decay >= 0 && eps >= 0, "adamw_step: lr, weight_decay and eps must not be negative");
   TORCH_CHECK(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, "adamw_step: betas must be in [0, 1)");
   TORCH_CHECK(step_at || step >= 1, "adamw_step: step counts from 1");
   TORCH_CHECK(!lr_at || step_at, "adamw_step: lr on the device needs step there too");
   if (n == 0) return;
-  const bool eight = m_scales.has_value();
+  const bool eight = (bool)m_scales;
   const auto state = eight ? torch::kFloat8_e4m3fn : torch::kFloat;
+  const Tensor &like = params[0];
   struct Group {
     int dtype, grad_dtype;
     bool master;
@@ -382,75 +410,75 @@ void adamw_step(const Tensors &params, const Tensors &grads, const Tensors &m, c
   std::vector<Group> groups;
   std::vector<const void *> seen;
   seen.reserve(n);
+  const auto fits = [&](const Tensor &t, const char *name, torch::ScalarType type, int64_t numel) -> void * {
+    TORCH_CHECK(t.scalar_type() == type, name, " must be ", type, ", got ", t.scalar_type());
+    TORCH_CHECK(t.layout() == torch::kStrided && t.is_contiguous(), name, " must be contiguous");
+    TORCH_CHECK(t.numel() == numel, name, " must have ", numel, " values, got ", t.numel());
+    return t.unsafeGetTensorImpl()->mutable_data();
+  };
+  // (sizes and types of all first: these refusals need no device)
   for (size_t i = 0; i < n; i++) {
     const Tensor &p = params[i], &g = grads[i];
     const int dtype = element_of(p, "param"), grad_dtype = element_of(g, "grad");
-    const bool master = masters && (*masters)[i].has_value();
+    const bool master = masters && masters.has(i);
     TORCH_CHECK(grad_dtype == dtype || grad_dtype == SPH_F32, "grad must be float32 or have its param's dtype");
     TORCH_CHECK(!master || dtype != SPH_F32, "a float32 param takes no master");
-    const int64_t blocks = (p.numel() + 255) / 256;
-    const auto fits = [&](const Tensor &t, const char *name, torch::ScalarType type, int64_t numel) {
-      TORCH_CHECK(t.scalar_type() == type, name, " must be ", type, ", got ", t.scalar_type());
-      TORCH_CHECK(t.numel() == numel, name, " must have ", numel, " values, got ", t.numel());
-      TORCH_CHECK(t.layout() == torch::kStrided && t.is_contiguous(), name, " must be contiguous");
-    };
-    fits(p, "param", p.scalar_type(), p.numel());
-    fits(g, "grad", g.scalar_type(), p.numel());
-    fits(m[i], "exp_avg", state, p.numel());
-    fits(v[i], "exp_avg_sq", state, p.numel());
-    if (master) fits(*(*masters)[i], "master", torch::kFloat, p.numel());
-    if (eight) {
-      fits((*m_scales)[i], "exp_avg_scale", torch::kFloat, blocks);
-      fits((*v_scales)[i], "exp_avg_sq_scale", torch::kFloat, blocks);
-    }
-    for (const Tensor *t : {&p, &g, &m[i], &v[i]}) check_device(*t, "every tensor of adamw_step", params[0]);
-    if (master) check_device(*(*masters)[i], "master", params[0]);
-    if (eight)
-      for (const Tensor *t : {&(*m_scales)[i], &(*v_scales)[i]}) check_device(*t, "scale", params[0]);
-    if (p.numel() == 0) continue;
-    seen.push_back(p.data_ptr());
+    const int64_t numel = p.numel(), blocks = (numel + 255) / 256;
     size_t at = 0;
     while (at < groups.size() && !(groups[at].dtype == dtype && groups[at].grad_dtype == grad_dtype && groups[at].master == master)) at++;
     if (at == groups.size()) {
       groups.emplace_back();
-      groups[at].dtype = dtype, groups[at].grad_dtype = grad_dtype, groups[at].master = master;
+      Group &q = groups[at];
+      q.dtype = dtype, q.grad_dtype = grad_dtype, q.master = master;
+      q.p.reserve(n), q.g.reserve(n), q.m.reserve(n), q.v.reserve(n), q.n.reserve(n);
+      if (master) q.w.reserve(n);
+      if (eight) q.ms.reserve(n), q.vs.reserve(n);
     }
     Group &q = groups[at];
-    q.p.push_back(p.data_ptr()), q.g.push_back(g.data_ptr()), q.m.push_back(m[i].data_ptr()), q.v.push_back(v[i].data_ptr());
-    q.n.push_back(p.numel());
-    if (master) q.w.push_back((*masters)[i]->data_ptr<float>());
-    if (eight) q.ms.push_back((*m_scales)[i].data_ptr<float>()), q.vs.push_back((*v_scales)[i].data_ptr<float>());
+    q.p.push_back(fits(p, "param", p.scalar_type(), numel));
+    q.g.push_back(fits(g, "grad", g.scalar_type(), numel));
+    q.m.push_back(fits(m[i], "exp_avg", state, numel));
+    q.v.push_back(fits(v[i], "exp_avg_sq", state, numel));
+    q.n.push_back(numel);
+    if (master) q.w.push_back((float *)fits(masters[i], "master", torch::kFloat, numel));
+    if (eight) {
+      q.ms.push_back((float *)fits(m_scales[i], "exp_avg_scale", torch::kFloat, blocks));
+      q.vs.push_back((float *)fits(v_scales[i], "exp_avg_sq_scale", torch::kFloat, blocks));
+    }
+    if (numel > 0) seen.push_back(q.p.back());
   }
-  std::sort(seen.begin(), seen.end());
-  TORCH_CHECK(std::adjacent_find(seen.begin(), seen.end()) == seen.end(), "adamw_step: a param appears twice");
   const auto scalar = [&](const OptTensor &t, const char *name) -> const float * {
     if (!t) return nullptr;
     TORCH_CHECK(t->scalar_type() == torch::kFloat && t->numel() == 1, name, " must be one float32 value");
-    check_device(*t, name, params[0]);
+    check_device(*t, name, like);
     return t->data_ptr<float>();
   };
   const float *step_p = scalar(step_at, "step"), *lr_p = scalar(lr_at, "lr");
-  c10::cuda::CUDAGuard guard(params[0].device());
+  const c10::Device device = like.device();
+  const TensorList *lists[] = {&params, &grads, &m, &v, &masters, &m_scales, &v_scales};
+  for (const TensorList *list : lists)
+    for (size_t i = 0; *list && i < n; i++)
+      if (list->has(i)) {
+        const Tensor &t = (*list)[i];
+        TORCH_CHECK(t.is_cuda() && t.device() == device, "every tensor of adamw_step must be a CUDA tensor of one device (this build has no CPU path)");
+      }
+  std::sort(seen.begin(), seen.end());
+  TORCH_CHECK(std::adjacent_find(seen.begin(), seen.end()) == seen.end(), "adamw_step: a param appears twice");
+  c10::cuda::CUDAGuard guard(device);
   for (Group &q : groups)
     ok(sph_adamw_step((int64_t)q.n.size(), q.p.data(), q.g.data(), q.master ? q.w.data() : nullptr, q.m.data(), q.v.data(),
                       eight ? q.ms.data() : nullptr, eight ? q.vs.data() : nullptr, q.n.data(), q.dtype, q.grad_dtype, eight ? 8 : 32, lr,
                       beta1, beta2, eps, weight_decay, grad_scale, step, lr_p, step_p, current_stream()),
        "sph_adamw_step");
   // written behind autograd's back: whoever saved one of these tensors has to notice
-  const auto touched = [](const Tensor &t) {
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-  };
-  for (size_t i = 0; i < n; i++) {
-    touched(params[i]), touched(m[i]), touched(v[i]);
-    if (masters && (*masters)[i]) touched(*(*masters)[i]);
-    if (eight) touched((*m_scales)[i]), touched((*v_scales)[i]);
-  }
+  for (const TensorList *list : lists)
+    for (size_t i = 0; list != &grads && *list && i < n; i++)
+      if (list->has(i) && !(*list)[i].is_inference()) (*list)[i].unsafeGetTensorImpl()->bump_version();
 }
 
 }  // namespace
 
 void bind_network_ops(pybind11::module_ &m) {
-  namespace py = pybind11;
   m.def("rms_norm_op", &rms_norm, py::arg("x"), py::arg("weight"), py::arg("residual"), py::arg("eps"), py::arg("dim"),
         py::arg("inside") = false);
   m.def("rms_norm_quantized", &rms_norm_quantized, py::arg("x"), py::arg("weight"), py::arg("residual"), py::arg("eps"), py::arg("dim"));
