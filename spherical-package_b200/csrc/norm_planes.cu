@@ -4,9 +4,9 @@
 
 namespace sph {
 
-template <typename T, bool E4M3, bool ADD, int MODE, int LOG> __global__ void __launch_bounds__(kPlaneThreads, 4) norm_planes_kernel(NormArgs a, PlaneTile tile) {
-  using L = Lane<T, MODE, LOG>;
-  using G = Geometry<T, MODE, LOG>;
+template <typename T, bool E4M3, bool ADD, int MODE, int LOG, int U> __global__ void __launch_bounds__(kPlaneThreads, 4) norm_planes_kernel(NormArgs a, PlaneTile tile) {
+  using L = Lane<T, MODE, LOG, U>;
+  using G = Geometry<T, MODE, LOG, U>;
   constexpr int N = L::N;
   __shared__ float shared[2][kPlaneThreads * N];
   __shared__ float weight[kMostPlanes];
@@ -14,39 +14,37 @@ template <typename T, bool E4M3, bool ADD, int MODE, int LOG> __global__ void __
   const int first = (threadIdx.x >> 5) & (ACROSS - 1);
   const Run<MODE, G::PIXELS> run(tile, blockIdx.x, a.outer, a.C, a.inner);
   T *s = (T *)plane_memory, *add = s + a.C * G::PITCH;
-  copy_run<T, MODE, LOG>(s, (const T *)a.x, run);
-  if (ADD) copy_run<T, MODE, LOG>(add, (const T *)a.residual, run);
+  copy_run<T, MODE, LOG, U>(s, (const T *)a.x, run);
+  if (ADD) copy_run<T, MODE, LOG, U>(add, (const T *)a.residual, run);
   copies_end();
   keep_weights<T>(weight, a.weight, a.weight_f32, a.C);
   const L px(run, first);
-  const int64_t step = ACROSS * a.inner;
-  const int shift = MODE == kShifted ? shift_of((const T *)a.x + run.offset(0), 0, first, a.inner) : 0;
-  T *mine = s + first * G::PITCH + px.col + shift;
-  const T *other = ADD ? add + first * G::PITCH + px.col + (MODE == kShifted ? shift_of((const T *)a.residual + run.offset(0), 0, first, a.inner) : 0) : nullptr;
+  const int64_t step = ACROSS * a.inner, zero = MODE == kShifted ? run.offset(0) : 0;
+  const Rows<T, MODE, LOG, U> mine(s, (const T *)a.x, zero, first, px.col, a.inner);
+  const Rows<T, MODE, LOG, U> other(add, (const T *)(ADD ? a.residual : a.x), zero, first, px.col, a.inner);
+  const int count = (a.C - first + ACROSS - 1) >> LOG;  // channels of this warp
+  const float *w = weight + first;
   copies_wait<0>();
   __syncthreads();
   float v[N], most[N];  // sums of squares; largest |s w|
 #pragma unroll
   for (int i = 0; i < N; i++) v[i] = most[i] = 0.f;
-  {
-    T *p = mine;
-    int64_t plane = 0;
+  int64_t plane = 0;
 #pragma unroll 8
-    for (int c = first; c < a.C; c += ACROSS, p += G::ROW, plane += step) {
-      Pixels<T> q = L::load(p);
-      if (ADD) {
-        const Pixels<T> o = L::load(other + (p - mine));
+  for (int k = 0; k < count; k++, plane += step) {
+    typename L::P q = L::load(mine(k));
+    if (ADD) {
+      const typename L::P o = L::load(other(k));
 #pragma unroll
-        for (int i = 0; i < N; i++) q.t[i] = from_float<T>(to_float(q.t[i]) + to_float(o.t[i]));
-        L::keep(p, q);
-        px.store((T *)a.sum, plane, q);
-      }
+      for (int i = 0; i < N; i++) q.t[i] = from_float<T>(to_float(q.t[i]) + to_float(o.t[i]));
+      L::keep(mine(k), q);
+      px.store((T *)a.sum, plane, q);
+    }
 #pragma unroll
-      for (int i = 0; i < N; i++) {
-        const float f = to_float(q.t[i]);
-        v[i] = fmaf(f, f, v[i]);
-        if (E4M3) most[i] = max_nan(most[i], fabsf(f * weight[c]));
-      }
+    for (int i = 0; i < N; i++) {
+      const float f = to_float(q.t[i]);
+      v[i] = fmaf(f, f, v[i]);
+      if (E4M3) most[i] = max_nan(most[i], fabsf(f * w[k * ACROSS]));
     }
   }
   plane_join<LOG>(v, shared[0], [](float p, float q) { return p + q; });
@@ -62,14 +60,13 @@ template <typename T, bool E4M3, bool ADD, int MODE, int LOG> __global__ void __
       scale[i] = rstd[i] * sc.inverse;
     }
   }
-  const T *p = mine;
-  int64_t plane = 0;
+  plane = 0;
 #pragma unroll 8
-  for (int c = first; c < a.C; c += ACROSS, p += G::ROW, plane += step) {
-    Pixels<T> q = L::load(p);
+  for (int k = 0; k < count; k++, plane += step) {
+    typename L::P q = L::load(mine(k));
     float y[N];
 #pragma unroll
-    for (int i = 0; i < N; i++) y[i] = to_float(q.t[i]) * (E4M3 ? scale[i] : rstd[i]) * weight[c];
+    for (int i = 0; i < N; i++) y[i] = to_float(q.t[i]) * (E4M3 ? scale[i] : rstd[i]) * w[k * ACROSS];
     if (E4M3) {
       px.store_e4m3((__nv_fp8_storage_t *)a.out, plane, y);
     } else {
@@ -85,9 +82,9 @@ template <typename T, bool E4M3> void norm_planes_launch(const NormArgs &a, cuda
   SPH_DISPATCH_PLANES(mode, a.C, {
     const PlaneTile tile = PlaneTile::of<G, MODE>(a.outer, a.inner);
     if (a.residual)
-      plane_launch<G, T>(norm_planes_kernel<T, E4M3, true, MODE, LOG>, a, tile, 2, (unsigned)tile.runs, st);
+      plane_launch<G, T>(norm_planes_kernel<T, E4M3, true, MODE, LOG, U>, a, tile, 2, (unsigned)tile.runs, st);
     else
-      plane_launch<G, T>(norm_planes_kernel<T, E4M3, false, MODE, LOG>, a, tile, 1, (unsigned)tile.runs, st);
+      plane_launch<G, T>(norm_planes_kernel<T, E4M3, false, MODE, LOG, U>, a, tile, 1, (unsigned)tile.runs, st);
   })
 }
 

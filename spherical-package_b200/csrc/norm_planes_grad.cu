@@ -6,10 +6,10 @@ namespace sph {
 
 // Backward: the blocks walk over the runs of pixels; a warp's channels, up to K, stay the same, and its lanes keep their parts of
 // the weight gradients in registers.
-template <typename T, int K, bool ADD, int MODE, int LOG>
+template <typename T, int K, bool ADD, int MODE, int LOG, int U>
 __global__ void __launch_bounds__(kPlaneThreads, K <= 32 ? 3 : 2) norm_planes_grad_kernel(NormGradArgs a, PlaneTile tile) {
-  using L = Lane<T, MODE, LOG>;
-  using G = Geometry<T, MODE, LOG>;
+  using L = Lane<T, MODE, LOG, U>;
+  using G = Geometry<T, MODE, LOG, U>;
   constexpr int N = L::N, ACROSS = G::ACROSS;
   __shared__ float shared[2][kPlaneThreads * N];
   __shared__ float weight[kMostPlanes];
@@ -24,10 +24,10 @@ __global__ void __launch_bounds__(kPlaneThreads, K <= 32 ? 3 : 2) norm_planes_gr
   int turn = 0;
   for (int64_t index = blockIdx.x; index < tile.runs; index += gridDim.x, turn ^= 1) {
     const Run<MODE, G::PIXELS> run(tile, index, a.outer, a.C, a.inner);
-    copy_run<T, MODE, LOG>(s, (const T *)a.s, run);
-    copy_run<T, MODE, LOG>(g, (const T *)a.gout, run);
+    copy_run<T, MODE, LOG, U>(s, (const T *)a.s, run);
+    copy_run<T, MODE, LOG, U>(g, (const T *)a.gout, run);
     copies_end();
-    if (ADD && a.gx) copy_run<T, MODE, LOG>(add, (const T *)a.gsum, run);
+    if (ADD && a.gx) copy_run<T, MODE, LOG, U>(add, (const T *)a.gsum, run);
     copies_end();
     const L px(run, first);
     float rstd[N], dot[N];
@@ -36,13 +36,12 @@ __global__ void __launch_bounds__(kPlaneThreads, K <= 32 ? 3 : 2) norm_planes_gr
       rstd[i] = px.in[i] ? a.rstd[px.norm[i]] : 0.f;
       dot[i] = 0.f;
     }
-    const int at = first * G::PITCH + px.col;
     const int64_t zero = MODE == kShifted ? run.offset(0) : 0;
-    const T *sp = s + at + (MODE == kShifted ? shift_of((const T *)a.s, zero, first, a.inner) : 0);
-    const T *gp = g + at + (MODE == kShifted ? shift_of((const T *)a.gout, zero, first, a.inner) : 0);
-    const T *ap = add + at + (MODE == kShifted && ADD ? shift_of((const T *)a.gsum, zero, first, a.inner) : 0);
+    using R = Rows<T, MODE, LOG, U>;
+    const R sp(s, (const T *)a.s, zero, first, px.col, a.inner), gp(g, (const T *)a.gout, zero, first, px.col, a.inner),
+        ap(add, (const T *)(ADD ? a.gsum : a.gout), zero, first, px.col, a.inner);
     const auto take = [&](int k) {
-      const Pixels<T> p = L::load(sp + k * G::ROW), q = L::load(gp + k * G::ROW);
+      const typename L::P p = L::load(sp(k)), q = L::load(gp(k));
       const float w = weight[first + k * ACROSS];
 #pragma unroll
       for (int i = 0; i < N; i++) {
@@ -72,10 +71,10 @@ __global__ void __launch_bounds__(kPlaneThreads, K <= 32 ? 3 : 2) norm_planes_gr
       if (ADD) __syncthreads();
       const float *wp = weight + first;
       int64_t plane = 0;
-      const auto give = [&](int j) {
-        Pixels<T> p = L::load(sp + j * G::ROW), q = L::load(gp + j * G::ROW), r;
-        if (ADD) r = L::load(ap + j * G::ROW);
-        const float w = wp[j * ACROSS];
+      const auto give = [&](int k) {
+        typename L::P p = L::load(sp(k)), q = L::load(gp(k)), r;
+        if (ADD) r = L::load(ap(k));
+        const float w = wp[k * ACROSS];
 #pragma unroll
         for (int i = 0; i < N; i++) {
           const float v = fmaf(to_float(q.t[i]) * w, rstd[i], to_float(p.t[i]) * dot[i]);
@@ -84,14 +83,14 @@ __global__ void __launch_bounds__(kPlaneThreads, K <= 32 ? 3 : 2) norm_planes_gr
         px.store((T *)a.gx, plane, p);
         plane += step;
       };
-      int left = mine;
-      for (; left >= 8; left -= 8, sp += 8 * G::ROW, gp += 8 * G::ROW, ap += 8 * G::ROW, wp += 8 * ACROSS) {
+      int k = 0;
+      for (; k + 8 <= mine; k += 8) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) give(j);
+        for (int j = 0; j < 8; j++) give(k + j);
       }
 #pragma unroll
       for (int j = 0; j < 7; j++)
-        if (j < left) give(j);
+        if (k + j < mine) give(k + j);
     }
     __syncthreads();  // everybody is done with the run
   }
@@ -111,26 +110,30 @@ __global__ void __launch_bounds__(kPlaneThreads, K <= 32 ? 3 : 2) norm_planes_gr
   }
 }
 
-template <typename T, int K, int MODE, int LOG> void norm_planes_grad_launch(NormGradArgs &a, cudaStream_t st) {
-  using G = Geometry<T, MODE, LOG>;
+template <typename T, int K, int MODE, int LOG, int U> void norm_planes_grad_launch(NormGradArgs &a, cudaStream_t st) {
+  using G = Geometry<T, MODE, LOG, U>;
   const PlaneTile tile = PlaneTile::of<G, MODE>(a.outer, a.inner);
   // as many blocks as are on the SMs at once: three by their registers, or what shared memory leaves room for
   const int fit = 225 * 1024 / ((int)sizeof(T) * a.C * G::PITCH * (a.gsum ? 3 : 2) + 6 * 1024 + 1024);
   a.splits = (int)std::min<int64_t>(a.splits, std::min<int64_t>(tile.runs, 148 * (fit >= 3 && K <= 32 ? 3 : fit >= 2 ? 2 : 1)));
   if (a.gsum)
-    plane_launch<G, T>(norm_planes_grad_kernel<T, K, true, MODE, LOG>, a, tile, 3, a.splits, st);
+    plane_launch<G, T>(norm_planes_grad_kernel<T, K, true, MODE, LOG, U>, a, tile, 3, a.splits, st);
   else
-    plane_launch<G, T>(norm_planes_grad_kernel<T, K, false, MODE, LOG>, a, tile, 2, a.splits, st);
+    plane_launch<G, T>(norm_planes_grad_kernel<T, K, false, MODE, LOG, U>, a, tile, 2, a.splits, st);
 }
 
 void norm_planes_backward(NormGradArgs &a, int dtype, cudaStream_t st) {
   SPH_DISPATCH_ELEMENT(dtype, {
     const Mode mode = plane_mode<T>(a.C, a.inner, planes_aligned<T>(a.inner, {a.s, a.gout, a.gsum, a.gx}));
     SPH_DISPATCH_PLANES(mode, a.C, {
-      if (LOG == 0 || a.C <= 256)
-        norm_planes_grad_launch<T, 32, MODE, LOG>(a, st);
-      else if constexpr (LOG == 3)
-        norm_planes_grad_launch<T, 64, MODE, LOG>(a, st);
+      if constexpr (U == 2)
+        norm_planes_grad_launch<T, kTwice / 8, MODE, LOG, U>(a, st);
+      else if constexpr (LOG == 0)
+        norm_planes_grad_launch<T, kAlone, MODE, LOG, U>(a, st);
+      else if (a.C <= 256)
+        norm_planes_grad_launch<T, 32, MODE, LOG, U>(a, st);
+      else
+        norm_planes_grad_launch<T, 64, MODE, LOG, U>(a, st);
     })
   });
 }

@@ -18,16 +18,16 @@ namespace sph {
 //            boundary as in its tensor; a lane has every 32nd pixel, and a run stays in its image;
 //   kSingle  pixel by pixel (small images, few channels).
 enum Mode { kWide, kShifted, kSingle };
-template <typename T> union Pixels {  // a lane's, of a channel
-  static constexpr int N = 4 / (int)sizeof(T), V = 16 / (int)sizeof(T);
-  unsigned w;
+template <typename T, int U> union Pixels {  // a lane's, of a channel: 4 or 8 bytes
+  static constexpr int N = 4 * U / (int)sizeof(T);
+  unsigned w[U];
   T t[N];
   __device__ __forceinline__ Pixels() {}
 };
 constexpr int kPlaneWarps = 8, kPlaneThreads = 32 * kPlaneWarps, kMostPlanes = 512;
-// LOG: log2 of the warps that share a unit's channels, 0 (one warp has them all) or 3.
-template <typename T, int MODE, int LOG> struct Geometry {
-  static constexpr int N = Pixels<T>::N, V = Pixels<T>::V;
+// LOG: log2 of the warps that share a unit's channels, 0 (one warp has them all) or 3.  U: 4-byte parts of a lane.
+template <typename T, int MODE, int LOG, int U> struct Geometry {
+  static constexpr int N = Pixels<T, U>::N, V = 16 / (int)sizeof(T);
   static constexpr int ACROSS = 1 << LOG, PIXELS = 256 * N >> LOG;  // of a run
   static constexpr int PITCH = PIXELS + (MODE == kShifted ? V : 0);  // elements from a channel's row to the next
   static constexpr int ROW = ACROSS * PITCH;                         // to a warp's next channel
@@ -45,12 +45,14 @@ struct PlaneTile {
     return t;
   }
 };
-// Channels one warp may have alone; with more, eight share them.
-constexpr int kAlone = 32;
+// Channels one warp may have alone; with more, eight share them; and up to which a lane has eight bytes of each, so that what
+// a run costs whatever its channels spreads over more pixels (8-bit norms of 3 x 96 x 181 x 333 bf16 28.7 us with four, 24.9 with
+// eight).
+constexpr int kAlone = 32, kTwice = 128;
 // Runs that end with their image are to be an eighth more at most.
 template <typename T> Mode plane_mode(int64_t C, int64_t inner, bool aligned) {
-  using G = Geometry<T, kShifted, 3>;
-  return aligned ? kWide : C > kAlone && 8 * ((inner + G::PIXELS - 1) / G::PIXELS * G::PIXELS) <= 9 * inner ? kShifted : kSingle;
+  const int64_t pixels = C > kAlone ? Geometry<T, kShifted, 3, 1>::PIXELS : Geometry<T, kShifted, 0, 1>::PIXELS;
+  return aligned ? kWide : 8 * ((inner + pixels - 1) / pixels * pixels) <= 9 * inner ? kShifted : kSingle;
 }
 
 // A run of pixels: offset of channel 0 of its pixel i, and the norms' numbers.
@@ -79,12 +81,28 @@ template <int MODE, int PIXELS> struct Run {
 
 // Elements between the 16-byte boundary before a channel's run and the run (kShifted), the same for a warp's channels.
 template <typename T> __device__ __forceinline__ int shift_of(const T *from, int64_t offset, int c, int64_t inner) {
-  return (int)(((uintptr_t)(from + offset) / sizeof(T) + (uintptr_t)c * (uintptr_t)inner) & (Pixels<T>::V - 1));
+  return (int)(((uintptr_t)(from + offset) / sizeof(T) + (uintptr_t)c * (uintptr_t)inner) & (16 / sizeof(T) - 1));
 }
 
+// Where a lane finds its pixels of a warp's k-th channel in shared memory.  A row's shift is the same for all channels of one of
+// eight warps (every eighth, and shifts repeat every V at the latest), and another for each of a warp's alone.
+template <typename T, int MODE, int LOG, int U> struct Rows {
+  using G = Geometry<T, MODE, LOG, U>;
+  T *base;
+  int shift, step;
+  __device__ __forceinline__ Rows(T *tile, const T *from, int64_t offset, int first, int col, int64_t inner) : base(tile + first * G::PITCH + col) {
+    shift = MODE == kShifted ? shift_of(from, offset, first, inner) : 0;
+    step = (int)(inner & (G::V - 1));
+    if (LOG == 3) base += shift;
+  }
+  __device__ __forceinline__ T *operator()(int k) const {
+    return base + k * G::ROW + (MODE == kShifted && LOG == 0 ? (shift + k * step) & (G::V - 1) : 0);
+  }
+};
+
 // Copies a run, all channels.
-template <typename T, int MODE, int LOG, class R> __device__ __forceinline__ void copy_run(T *to, const T *from, const R &run) {
-  using G = Geometry<T, MODE, LOG>;
+template <typename T, int MODE, int LOG, int U, class R> __device__ __forceinline__ void copy_run(T *to, const T *from, const R &run) {
+  using G = Geometry<T, MODE, LOG, U>;
   constexpr int V = G::V;
   if constexpr (MODE == kWide) {
     constexpr int COLS = G::PIXELS / V, ROWS = kPlaneThreads / COLS;
@@ -141,8 +159,9 @@ template <typename T, int MODE, int LOG, class R> __device__ __forceinline__ voi
 }
 
 // A lane's pixels of a run: col, col + 1 (kWide) or col, col + 32.
-template <typename T, int MODE, int LOG> struct Lane {
-  static constexpr int N = Pixels<T>::N, STEP = MODE == kWide ? 1 : 32;
+template <typename T, int MODE, int LOG, int U> struct Lane {
+  using P = Pixels<T, U>;
+  static constexpr int N = P::N, STEP = MODE == kWide ? 1 : 32;
   int col;
   bool in[N];
   int64_t norm[N], off[N];  // of the warp's first channel
@@ -158,26 +177,40 @@ template <typename T, int MODE, int LOG> struct Lane {
   }
   // (The pixels of a shifted run are in one image.)
   __device__ __forceinline__ int64_t at(int i) const { return MODE == kShifted ? off[0] + i * STEP : off[i]; }
-  static __device__ __forceinline__ Pixels<T> load(const T *p) {
-    Pixels<T> v;
-    if (MODE == kWide) v.w = *(const unsigned *)p;
-    else {
+  static __device__ __forceinline__ void words(const T *p, P &v) {
+    if constexpr (U == 1) {
+      v.w[0] = *(const unsigned *)p;
+    } else {
+      const uint2 q = *(const uint2 *)p;
+      v.w[0] = q.x, v.w[1] = q.y;
+    }
+  }
+  static __device__ __forceinline__ void put_words(T *p, const P &v) {
+    if constexpr (U == 1) *(unsigned *)p = v.w[0];
+    else *(uint2 *)p = make_uint2(v.w[0], v.w[1]);
+  }
+  static __device__ __forceinline__ P load(const T *p) {
+    P v;
+    if constexpr (MODE == kWide) {
+      words(p, v);
+    } else {
 #pragma unroll
       for (int i = 0; i < N; i++) v.t[i] = p[i * STEP];
     }
     return v;
   }
-  static __device__ __forceinline__ void keep(T *p, const Pixels<T> &v) {
-    if (MODE == kWide) *(unsigned *)p = v.w;
-    else {
+  static __device__ __forceinline__ void keep(T *p, const P &v) {
+    if constexpr (MODE == kWide) {
+      put_words(p, v);
+    } else {
 #pragma unroll
       for (int i = 0; i < N; i++) p[i * STEP] = v.t[i];
     }
   }
   // `plane`: elements from the warp's first channel.
-  __device__ __forceinline__ void store(T *to, int64_t plane, const Pixels<T> &v) const {
-    if (MODE == kWide) {
-      if (in[0]) *(unsigned *)(to + off[0] + plane) = v.w;
+  __device__ __forceinline__ void store(T *to, int64_t plane, const P &v) const {
+    if constexpr (MODE == kWide) {
+      if (in[0]) put_words(to + off[0] + plane, v);
     } else {
 #pragma unroll
       for (int i = 0; i < N; i++)
@@ -185,10 +218,18 @@ template <typename T, int MODE, int LOG> struct Lane {
     }
   }
   __device__ __forceinline__ void store_e4m3(__nv_fp8_storage_t *to, int64_t plane, const float (&y)[N]) const {
-    if (MODE == kWide && N == 2) {
-      if (in[0]) *(__nv_fp8x2_storage_t *)(to + off[0] + plane) = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[N - 1]), __NV_SATFINITE, __NV_E4M3);
-    } else if (MODE == kWide) {
+    if constexpr (MODE == kWide && N == 1) {
       if (in[0]) to[off[0] + plane] = to_e4m3(y[0]);
+    } else if constexpr (MODE == kWide) {
+      if (in[0]) {
+        const unsigned a = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
+        if constexpr (N == 2) {
+          *(__nv_fp8x2_storage_t *)(to + off[0] + plane) = (__nv_fp8x2_storage_t)a;
+        } else {
+          const unsigned b = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
+          *(unsigned *)(to + off[0] + plane) = a | b << 16;
+        }
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < N; i++)
@@ -233,16 +274,20 @@ void plane_launch(void (*kernel)(A, PlaneTile), const A &a, const PlaneTile &til
   if (bytes > 32768) cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   kernel<<<blocks, kPlaneThreads, bytes, st>>>(a, tile);
 }
-// Run a statement with MODE, LOG and the geometry G.
-#define SPH_PLANES(M, L, ...) { constexpr int MODE = M, LOG = L; using G = Geometry<T, MODE, LOG>; __VA_ARGS__; }
+// Run a statement with MODE, LOG, U and the geometry G.
+#define SPH_PLANES(M, L, P, ...) { constexpr int MODE = M, LOG = L, U = P; using G = Geometry<T, MODE, LOG, U>; __VA_ARGS__; }
+#define SPH_PLANES_OF(M, C, ...)                                       \
+  if (C <= kTwice) SPH_PLANES(M, 3, 2, __VA_ARGS__)                    \
+  else SPH_PLANES(M, 3, 1, __VA_ARGS__)
 #define SPH_DISPATCH_PLANES(mode, C, ...)                              \
   if (C <= kAlone) {                                                   \
-    if (mode == kWide) SPH_PLANES(kWide, 0, __VA_ARGS__)               \
-    else SPH_PLANES(kSingle, 0, __VA_ARGS__)                           \
+    if (mode == kWide) SPH_PLANES(kWide, 0, 1, __VA_ARGS__)            \
+    else if (mode == kShifted) SPH_PLANES(kShifted, 0, 1, __VA_ARGS__) \
+    else SPH_PLANES(kSingle, 0, 1, __VA_ARGS__)                        \
   } else {                                                             \
-    if (mode == kWide) SPH_PLANES(kWide, 3, __VA_ARGS__)               \
-    else if (mode == kShifted) SPH_PLANES(kShifted, 3, __VA_ARGS__)    \
-    else SPH_PLANES(kSingle, 3, __VA_ARGS__)                           \
+    if (mode == kWide) { SPH_PLANES_OF(kWide, C, __VA_ARGS__) }        \
+    else if (mode == kShifted) { SPH_PLANES_OF(kShifted, C, __VA_ARGS__) } \
+    else { SPH_PLANES_OF(kSingle, C, __VA_ARGS__) }                    \
   }
 
 }  // namespace sph
