@@ -89,15 +89,14 @@ struct Stats {
     s += o.s;
     t += o.t;
   }
-  // Over the warp, the same in every lane.
-  __device__ __forceinline__ void join_warp() {
-    float n = m;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) n = max_nan(n, __shfl_xor_sync(0xffffffffu, n, d));
-    move_to(n);
-    s = warp_sum(s);
-    t = warp_sum(t);
+  // Over groups of `lanes` neighbouring lanes of the warp, the same in each.
+  __device__ __forceinline__ void join_lanes(int lanes) {
+    move_to(lanes_join(m, lanes, [](float a, float b) { return max_nan(a, b); }));
+    const auto add = [](float a, float b) { return a + b; };
+    s = lanes_join(s, lanes, add);
+    t = lanes_join(t, lanes, add);
   }
+  __device__ __forceinline__ void join_warp() { join_lanes(32); }
   __device__ __forceinline__ float entropy() const {
     const float h = s == 0.f ? 0.f : logf(s) - kLn2 * (t / s);
     return h < 0.f ? 0.f : h;
@@ -410,24 +409,27 @@ template <typename T> __global__ void __launch_bounds__(kStreamThreads, kStreamB
   }
 }
 
-// Rows of up to 1024 classes: a warp each, their logits in registers; the best by the same bound, of the maxima of the lanes.
-template <typename T, bool TOP> __global__ void __launch_bounds__(256, TOP ? 2 : 4) log_probs_warp_kernel(LogProbArgs a) {
-  constexpr int V = 32 / RowVector<T>::N, POOL = 96;
+// Rows of up to 1024 classes: a warp each (or `lanes` of one, a power of two, where no best are asked for), their logits in
+// registers; the best by the same bound, of the maxima of the lanes.
+template <typename T, bool TOP, int E> __global__ void __launch_bounds__(256, TOP ? 2 : 4) log_probs_warp_kernel(LogProbArgs a, int lanes) {
+  constexpr int V = E / RowVector<T>::N, POOL = 96;
   __shared__ Candidate pools[TOP ? 8 : 1][POOL];
   __shared__ int counts[8];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = (int64_t)blockIdx.x * 8 + warp;
-  if (row >= a.outer) return;
-  const T *x = (const T *)a.x + row * a.x_stride;
-  const int shift = RowVector<T>::shift_of(x), vectors = (a.C + shift + RowVector<T>::N - 1) / RowVector<T>::N;
+  if (TOP) lanes = 32;
+  const int lane = threadIdx.x & (lanes - 1), warp = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
+  const bool on = row < a.outer;
+  if (TOP && !on) return;
+  const T *x = (const T *)a.x + (on ? row : 0) * a.x_stride;
+  const int shift = RowVector<T>::shift_of(x), vectors = on ? (a.C + shift + RowVector<T>::N - 1) / RowVector<T>::N : 0;
   Tile<T, V> tile;
-  tile.load(x, lane, 32, vectors, shift, a.C);
-  const int64_t t = a.target[row];
+  tile.load(x, lane, lanes, vectors, shift, a.C);
+  const int64_t t = on ? a.target[row] : -1;
   const float x_t = t >= 0 && t < a.C ? to_float(x[t]) : 0.f, largest = tile.largest();
   Stats st;
   tile.add_to(st, largest);
-  st.join_warp();
-  if (lane == 0) write_stats(a, row, st, t, x_t);
+  st.join_lanes(lanes);
+  if (lane == 0 && on) write_stats(a, row, st, t, x_t);
   if (!TOP) return;
   const auto put = [&](int i, Candidate c) {
     a.top_index[row * a.k + i] = candidate_index(c);
@@ -817,6 +819,49 @@ template <typename T> void launch_planes_grad(const LogProbGradArgs &a, cudaStre
     log_probs_planes_grad_kernel<T, 1><<<(unsigned)((pixels + 127) / 128), 128, 0, st>>>(a, index);
 }
 
+// Rows of up to 1024 classes: `lanes` of a warp each.
+template <typename T> __global__ void __launch_bounds__(256) log_probs_warp_grad_kernel(LogProbGradArgs a, int lanes) {
+  constexpr int N = RowVector<T>::N;
+  const int lane = threadIdx.x & (lanes - 1);
+  const int64_t row = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
+  const bool on = row < a.outer;
+  const T *x = (const T *)a.x + (on ? row : 0) * a.x_stride;
+  T *gx = (T *)a.gx + (on ? row : 0) * a.C;
+  const RowGrad r = row_grad(a, on ? row : 0, on ? row : 0, 0);
+  const int shift = RowVector<T>::shift_of(gx), vectors = on ? (a.C + shift + N - 1) / N : 0;
+  const bool alike = RowVector<T>::shift_of(x) == shift;
+  const T none = from_float<T>(-INFINITY);
+  const int target = r.target >= 0 && r.target < a.C ? (int)r.target : -1;
+  for (int at = lane; at < vectors; at += lanes) {
+    const int first = at * N - shift;
+    RowVector<T> v;
+    if (alike) {
+      v.load(x, first, a.C, none);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; j++) v.t[j] = first + j >= 0 && first + j < a.C ? x[first + j] : none;
+    }
+    const bool here = target >= first && target < first + N;
+    const float g_t = here ? r.of(v.at_any(target - first)) + r.g : 0.f;
+#pragma unroll
+    for (int j = 0; j < N / 2; j++) v.set_pair(j, r.of(v.pair(j)));
+    if (here) v.set_any(target - first, g_t);
+    v.store(gx, first, a.C);
+  }
+  if (!a.t) return;
+  __syncwarp();
+  for (int j = lane; j < a.k && on && r.tops; j += lanes) {
+    const int64_t c = a.top_index[row * a.k + j];
+    if (c >= 0 && c < a.C) gx[c] = from_float<T>(r.of(to_float(x[c])) + own_grad(a, r, row, 0, (int)c));
+  }
+}
+// Lanes for a row: eight classes each, and what a row's start may take of a vector.
+template <typename T> int row_lanes(int64_t C) {
+  int n = 1;
+  while (n < 32 && 8 * n < C + RowVector<T>::N - 1) n *= 2;
+  return n;
+}
+
 // Blocks for a row: enough for two on each SM, no more than the row has tiles.
 inline int blocks_per_row(int64_t rows, int64_t C, int64_t tile, int most) {
   const int64_t tiles = (C + tile - 1) / tile;
@@ -826,7 +871,7 @@ inline int blocks_per_row(int64_t rows, int64_t C, int64_t tile, int most) {
 }
 // Rows as a grid's second and third dimension.
 inline dim3 row_grid(int n, int64_t rows) {
-  const unsigned y = rows < 32768 ? (unsigned)rows : 32768u;
+  const unsigned y = rows < 65535 ? (unsigned)rows : 65535u;
   return dim3((unsigned)n, y, (unsigned)((rows + y - 1) / y));
 }
 
@@ -880,9 +925,11 @@ extern "C" int sph_token_log_probs_forward(const void *x, const int64_t *target,
   cudaStream_t st = (cudaStream_t)stream;
   int launches = 1;
   SPH_DISPATCH_ELEMENT(dtype, {
-    if (inner == 1 && C <= 1024 - RowVector<T>::N)  // (a row's start may take a part of a vector)
-      (k > 0 ? log_probs_warp_kernel<T, true> : log_probs_warp_kernel<T, false>)<<<(unsigned)((outer + 7) / 8), 256, 0, st>>>(a);
-    else if (inner == 1 && k > kMostTop)
+    if (inner == 1 && C <= 1024 - RowVector<T>::N) {  // (a row's start may take a part of a vector)
+      const int lanes = k > 0 ? 32 : row_lanes<T>(C), rows = 256 / lanes;
+      // (a lane has 16 logits where 8 and a row's start are enough, else 32)
+      (k > 0 ? log_probs_warp_kernel<T, true, 32> : C <= 256 - RowVector<T>::N ? log_probs_warp_kernel<T, false, 16> : log_probs_warp_kernel<T, false, 32>)<<<(unsigned)((outer + rows - 1) / rows), 256, 0, st>>>(a, lanes);
+    } else if (inner == 1 && k > kMostTop)
       log_probs_many_kernel<T><<<(unsigned)outer, 256, 0, st>>>(a);
     else if (inner == 1) {
       if (launch_rows<T>(a, st) != cudaSuccess) {
@@ -910,7 +957,10 @@ extern "C" int sph_token_log_probs_backward(const void *x, const int64_t *target
                           (int)C, (int)k};
   cudaStream_t st = (cudaStream_t)stream;
   SPH_DISPATCH_ELEMENT(dtype, {
-    if (inner == 1)
+    if (inner == 1 && C <= 1024 - RowVector<T>::N) {
+      const int lanes = row_lanes<T>(C), rows = 256 / lanes;
+      log_probs_warp_grad_kernel<T><<<(unsigned)((outer + rows - 1) / rows), 256, 0, st>>>(a, lanes);
+    } else if (inner == 1)
       log_probs_rows_grad_kernel<T><<<row_grid(blocks_per_row(outer, C, 256 * RowVector<T>::N, 64), outer), 256, 0, st>>>(a);
     else
       launch_planes_grad<T>(a, st);

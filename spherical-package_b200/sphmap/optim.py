@@ -52,9 +52,11 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       master_weights=master_weights, capturable=capturable))
 
-    def _state_of(self, p, group):
+    def _state_of(self, p, group, capturing):
         s = self.state[p]
         if not s:
+            if capturing:
+                raise RuntimeError("AdamW: a step has to run before one is captured in a graph")
             if not p.is_contiguous():
                 raise RuntimeError("param must be contiguous")
             if not group["capturable"]:
@@ -80,7 +82,7 @@ class AdamW(torch.optim.Optimizer):
                     self.state[p][k] = v.detach().to(device=p.device, copy=True)
         for g in self.param_groups:
             if isinstance(g.get("step"), torch.Tensor):
-                g["step"] = g["step"].to(g["params"][0].device)
+                g["step"] = g["step"].detach().to(device=g["params"][0].device, copy=True)
 
     @torch.no_grad()
     def step(self, closure=None, grad_scale=1.0):
@@ -89,14 +91,17 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
         for group in self.param_groups:
+            if capturing and not group["capturable"]:
+                raise RuntimeError("AdamW: a captured step needs capturable=True (its number would stay what it was)")
             together = {}   # params at one step number: all, unless some had no gradient in an earlier step
             for p in group["params"]:
                 if p.grad is None:
                     continue
                 if p.grad.layout != torch.strided:
                     raise RuntimeError("gradients must be dense")
-                s = self._state_of(p, group)
+                s = self._state_of(p, group, capturing)
                 together.setdefault((p.device, s.get("step")), []).append((p, s))
             if group["capturable"] and together:
                 if len(together) > 1:

@@ -99,7 +99,7 @@ def test_adamw_state_dict_keeps_types():
     def filled():
         p = torch.zeros(300, dtype=torch.bfloat16, requires_grad=True)
         o = optim.AdamW([p], state_bits=8, master_weights=True)
-        o._state_of(p, o.param_groups[0])
+        o._state_of(p, o.param_groups[0], False)
         return p, o
     p, o = filled()
     s = o.state[p]

@@ -115,6 +115,16 @@ def test_norm_of_wider_rows_and_channels_last(c, dtype):
     check_quantized(img, w, img * 2, 1)
 
 
+def test_rows_that_are_a_first_dimension():
+    """(C, rows) over rows of C values: dimension 0 of a transposed tensor."""
+    x, r = normal((40, 72), 1).t(), normal((40, 72), 2).t()
+    w = normal((72,), 5) * 0.2 + 1
+    got = check_norm(x, w, r, 0, normal((72, 40), 3), normal((72, 40), 4))
+    assert got["out"].stride() == x.stride()
+    check_quantized(x, w, r, 0)
+    check_log_probs(x, torch.randint(72, (40,), generator=gen(1), device="cuda"), 0, 3)
+
+
 def test_norm_takes_shifted_addresses():
     """Contiguous tensors that start one value behind an aligned address."""
     for shape, dim in (((9, 512), -1), ((2, 64, 8, 16), 1)):
@@ -198,7 +208,7 @@ LOGPROB_SHAPES = [  # (shape, dim, ks)
     ((9, 1000), 1, (0, 8)), ((4, 1024), -1, (1, 20)), ((3, 1025), -1, (8,)), ((7, 4096), -1, (0, 2)), ((2, 4097), -1, (8,)),
     ((3, 8192), -1, (1,)), ((2, 16384), -1, (8,)), ((2, 16385), -1, (7,)), ((3, 32000), -1, (0, 20)), ((2, 50257), -1, (1, 33)),
     ((1, 131072), -1, (8,)), ((2, 131075), -1, (4,)), ((1, 300001), -1, (5,)), ((600, 1500), -1, (2,)), ((300, 70), -1, (3,)),
-    ((2, 3, 50), -1, (2,)), ((1, 13, 8, 16), 1, (0, 1, 4, 13)), ((2, 41, 11, 13), 1, (3, 20)), ((3, 2, 5), 1, (0, 2)), ((1, 150, 3, 64), 1, (8,)),
+    ((2, 3, 50), -1, (2,)), ((3001, 10), -1, (0, 3)), ((515, 64), -1, (0, 1)), ((260, 129), -1, (0,)), ((70, 1016), -1, (0, 9)), ((70, 1023), -1, (0,)), ((1, 13, 8, 16), 1, (0, 1, 4, 13)), ((2, 41, 11, 13), 1, (3, 20)), ((3, 2, 5), 1, (0, 2)), ((1, 150, 3, 64), 1, (8,)),
     ((1, 1, 4, 5), 1, (1,)), ((2, 300, 1, 7), 1, (9,)), ((4, 19, 64, 64), 1, (0, 5)), ((7, 3, 9), 0, (2,)), ((2, 1031, 2, 3), 1, (4,)),
     ((1, 5, 70000), 1, (0, 2)),
 ]
@@ -634,6 +644,33 @@ def test_mapped_network_step():
     for p, b, g in zip(params, before, got):
         z = torch.zeros_like(b)
         ref.close(p, *ref.adamw(b, g, z, z, 1, 1e-3, 0.9, 0.999, 1e-8, 0.01)[0], torch.float32, "param")
+
+
+def test_adamw_refuses_captures_that_would_not_count():
+    p = normal((100,), 1).requires_grad_()
+    p.grad = normal((100,), 2)
+    for o, message in ((optim.AdamW([p]), "capturable"), (optim.AdamW([p], capturable=True), "has to run before")):
+        with pytest.raises(RuntimeError, match=message):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                o.step()
+
+
+def test_capturable_step_and_lr_on_the_device():
+    a, b = normal((300,), 1).requires_grad_(), normal((300,), 1).requires_grad_()
+    lr = torch.tensor(1e-2, device="cuda")
+    o, o2 = optim.AdamW([a], lr=lr, capturable=True), optim.AdamW([b], lr=1e-2)
+    for i in range(3):
+        a.grad = b.grad = normal((300,), 10 + i)
+        o.step()
+        o2.step()
+    assert (a - b).abs().max() <= 3 * 1e-2 * 40 * ref.U + 4 * ref.U * b.abs().max()   # three steps of at most about lr each
+    c = a.detach().clone().requires_grad_()
+    o3 = optim.AdamW([c], lr=lr, capturable=True)
+    o3.load_state_dict(o.state_dict())
+    a.grad = c.grad = normal((300,), 20)
+    o.step()
+    o3.step()
+    assert torch.equal(a, c) and o3.param_groups[0]["step"].item() == 4 == o.param_groups[0]["step"].item()
 
 
 def test_shared_weight_sums_its_gradients():
