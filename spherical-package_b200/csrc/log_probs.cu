@@ -927,8 +927,8 @@ extern "C" int sph_token_log_probs_forward(const void *x, const int64_t *target,
   SPH_DISPATCH_ELEMENT(dtype, {
     if (inner == 1 && C <= 1024 - RowVector<T>::N) {  // (a row's start may take a part of a vector)
       const int lanes = k > 0 ? 32 : row_lanes<T>(C), rows = 256 / lanes;
-      // (a lane has 16 logits where 8 and a row's start are enough, else 32)
-      (k > 0 ? log_probs_warp_kernel<T, true, 32> : C <= 256 - RowVector<T>::N ? log_probs_warp_kernel<T, false, 16> : log_probs_warp_kernel<T, false, 32>)<<<(unsigned)((outer + rows - 1) / rows), 256, 0, st>>>(a, lanes);
+      // (a lane has 16 logits where those are enough, else 32)
+      (k > 0 ? log_probs_warp_kernel<T, true, 32> : C <= 512 - RowVector<T>::N ? log_probs_warp_kernel<T, false, 16> : log_probs_warp_kernel<T, false, 32>)<<<(unsigned)((outer + rows - 1) / rows), 256, 0, st>>>(a, lanes);
     } else if (inner == 1 && k > kMostTop)
       log_probs_many_kernel<T><<<(unsigned)outer, 256, 0, st>>>(a);
     else if (inner == 1) {

@@ -104,9 +104,11 @@ class EncoderStack:
     are allocated once; `step` enqueues one forward+backward pass and returns the loss tensor
     sum(out * grad_output) (device scalar).  With `fuse_relu` (default) the activation runs inside the
     convolution kernels (sph_mapped_conv_relu_*); without it as separate passes over the activations, the way the
-    reference's operators compose."""
+    reference's operators compose.  With `optimizer`, which makes a torch optimizer from the list of parameters (such as
+    `lambda p: sphmap.optim.AdamW(p, lr=1e-3)`), every step ends with an update of the weights and biases from the gradients
+    that the ranks have exchanged."""
 
-    def __init__(self, cfg, device, precision, local_batch, reducer=None, timers=None, fuse_relu=True, companions=None):
+    def __init__(self, cfg, device, precision, local_batch, reducer=None, timers=None, fuse_relu=True, companions=None, optimizer=None):
         from . import capi
         self.c = capi
         self.prec = precision
@@ -145,6 +147,14 @@ class EncoderStack:
         else:
             pairs = [(torch.empty(co, ci, self.K, **f32), torch.empty(co, **f32)) for ci, co, _, _, _ in self.layers]
         self.gw, self.gb = [p[0] for p in pairs], [p[1] for p in pairs]
+        self.optimizer = None if optimizer is None else optimizer(self.parameters())
+
+    def parameters(self):
+        """Weights and biases; the buffers that backward writes are their gradients."""
+        params = [t for pair in zip(self.w, self.b) for t in pair]
+        for p, g in zip(params, (g for pair in zip(self.gw, self.gb) for g in pair)):
+            p.grad = g
+        return params
 
     def _timed(self, key, fn):
         if self.timers is not None and key in self.timers:
@@ -232,4 +242,6 @@ class EncoderStack:
         out = self.forward(x)
         loss = torch.dot(out.reshape(-1), go.reshape(-1))   # sum(out * go) in one pass, without the product tensor
         self.backward(go)
+        if self.optimizer is not None:
+            self.optimizer.step()
         return loss

@@ -646,6 +646,23 @@ def test_mapped_network_step():
         ref.close(p, *ref.adamw(b, g, z, z, 1, 1e-3, 0.9, 0.999, 1e-8, 0.01)[0], torch.float32, "param")
 
 
+@pytest.mark.parametrize("precision", [0, 1])
+def test_encoder_stack_with_an_optimizer(precision):
+    """The encoder's step ends with AdamW's update from the gradients it left in its buffers."""
+    from sphmap import workloads
+    from sphmap.parallel import EncoderStack, GradReducer
+    cfg = workloads.config4(B=2, H=64, W=128)
+    x, go = cfg["x"].cuda(), cfg["grad_output"].cuda()
+    plain = EncoderStack(cfg, "cuda", precision, 2, GradReducer())
+    stack = EncoderStack(cfg, "cuda", precision, 2, GradReducer(), optimizer=lambda p: optim.AdamW(p, lr=1e-3))
+    loss = stack.step(x, go)
+    assert torch.equal(loss, plain.step(x, go))
+    for p, before, g in zip(stack.parameters(), plain.parameters(), (t for pair in zip(plain.gw, plain.gb) for t in pair)):
+        z = torch.zeros_like(p)
+        ref.close(p, *ref.adamw(before, g, z, z, 1, 1e-3, 0.9, 0.999, 1e-8, 0.01)[0], torch.float32, "parameter")
+    assert not torch.equal(stack.step(x, go), loss)
+
+
 def test_adamw_refuses_captures_that_would_not_count():
     p = normal((100,), 1).requires_grad_()
     p.grad = normal((100,), 2)
