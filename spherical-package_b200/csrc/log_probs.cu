@@ -563,20 +563,26 @@ template <int K> struct Best {
   }
 };
 
-constexpr int kPlaneChannels = 8;  // read at once
+// Channels read at once: by a thread of one pixel, which has fewer bytes on their way, twice as many.
+template <int P> constexpr int plane_channels() { return P == 1 ? 16 : 8; }
 
-// A thread has P pixels and walks over their channels, eight at a time; with K > 0 it keeps the K best of them on the way.
+// A thread has P pixels and walks over their channels, some at a time; with K > 0 it keeps the K best of them on the way.
 template <typename T, int P, int K> __global__ void __launch_bounds__(128) log_probs_planes_kernel(LogProbArgs a, PlaneIndex index) {
+  constexpr int CHANNELS = plane_channels<P>();
   const int64_t at = ((int64_t)blockIdx.x * 128 + threadIdx.x) * P;
   if (at >= a.outer * a.inner) return;
   const int64_t o = index.image(at), i = at - o * a.inner;
   const T *x = (const T *)a.x + o * a.C * a.inner + i;
   Stats st[P];
   Best<K ? K : 1> best[P];
-  for (int c0 = 0; c0 < a.C; c0 += kPlaneChannels) {
-    PixelVector<T, P> v[kPlaneChannels];
+  int64_t target[P];
+  float x_t[P];  // the target's logit, found on the way
 #pragma unroll
-    for (int c = 0; c < kPlaneChannels; c++) {
+  for (int p = 0; p < P; p++) target[p] = a.target[at + p], x_t[p] = 0.f;
+  for (int c0 = 0; c0 < a.C; c0 += CHANNELS) {
+    PixelVector<T, P> v[CHANNELS];
+#pragma unroll
+    for (int c = 0; c < CHANNELS; c++) {
       if (c0 + c < a.C) {
         v[c].load(x + (c0 + c) * a.inner);
       } else {
@@ -588,22 +594,22 @@ template <typename T, int P, int K> __global__ void __launch_bounds__(128) log_p
     for (int p = 0; p < P; p++) {
       float m = st[p].m;
 #pragma unroll
-      for (int c = 0; c < kPlaneChannels; c++) m = max_nan(m, to_float(v[c].t[p]));
+      for (int c = 0; c < CHANNELS; c++) m = max_nan(m, to_float(v[c].t[p]));
       st[p].move_to(m);
       const float base = Stats::base(m);
 #pragma unroll
-      for (int c = 0; c < kPlaneChannels; c++) {
+      for (int c = 0; c < CHANNELS; c++) {
         const float d = distance(to_float(v[c].t[p]), base), e = exp2_fast(d);
         st[p].s += e;
         st[p].t = fmaf(e, d, st[p].t);
+        if (c0 + c == (int)target[p]) x_t[p] = to_float(v[c].t[p]);  // (a target beyond 32 bits is none of the classes, and its logit not looked at)
         if (K > 0 && c0 + c < a.C) best[p].take(order_of(to_float(v[c].t[p])), c0 + c);
       }
     }
   }
 #pragma unroll
   for (int p = 0; p < P; p++) {
-    const int64_t t = a.target[at + p];
-    write_stats(a, at + p, st[p], t, t >= 0 && t < a.C ? to_float(x[t * a.inner + p]) : 0.f);
+    write_stats(a, at + p, st[p], target[p], x_t[p]);
 #pragma unroll
     for (int j = 0; j < K; j++)
       if (j < a.k) {
@@ -650,17 +656,19 @@ template <typename T, int P> void launch_planes(const LogProbArgs &a, cudaStream
     log_probs_planes_kernel<T, P, 0><<<blocks, 128, 0, st>>>(a, index);
   else if (a.k == 1)
     log_probs_planes_kernel<T, P, 1><<<blocks, 128, 0, st>>>(a, index);
-  else if (a.k <= 4)
-    log_probs_planes_kernel<T, P, 4><<<blocks, 128, 0, st>>>(a, index);
-  else
-    log_probs_planes_kernel<T, P, 8><<<blocks, 128, 0, st>>>(a, index);
+  else if constexpr (P == 1) {  // (lists of four pixels would not fit the registers)
+    if (a.k <= 4)
+      log_probs_planes_kernel<T, P, 4><<<blocks, 128, 0, st>>>(a, index);
+    else
+      log_probs_planes_kernel<T, P, 8><<<blocks, 128, 0, st>>>(a, index);
+  }
 }
 template <typename T> bool planes_of_four(int64_t inner, const void *x, const void *gx = nullptr) {
   return inner % 4 == 0 && ((uintptr_t)x | (uintptr_t)gx) % (4 * sizeof(T)) == 0;
 }
 // Kernels launched.
 template <typename T> int launch_planes(const LogProbArgs &a, cudaStream_t st) {
-  if (planes_of_four<T>(a.inner, a.x) && a.k <= 1)  // (lists of four pixels would not fit the registers)
+  if (planes_of_four<T>(a.inner, a.x) && a.k <= 1)
     launch_planes<T, 4>(a, st);
   else
     launch_planes<T, 1>(a, st);
@@ -773,11 +781,19 @@ template <typename T> __global__ void __launch_bounds__(256) log_probs_rows_grad
 
 // A thread has P pixels, as in the forward pass.
 template <typename T, int P> __global__ void __launch_bounds__(128) log_probs_planes_grad_kernel(LogProbGradArgs a, PlaneIndex index) {
+  constexpr int CHANNELS = plane_channels<P>();
   const int64_t at = ((int64_t)blockIdx.x * 128 + threadIdx.x) * P;
   if (at >= a.outer * a.inner) return;
   const int64_t o = index.image(at), i = at - o * a.inner, base = o * a.C * a.inner + i;
   const T *x = (const T *)a.x + base;
   T *gx = (T *)a.gx + base;
+  PixelVector<T, P> v[CHANNELS];
+  const auto read = [&](int c0) {
+#pragma unroll
+    for (int c = 0; c < CHANNELS; c++)
+      if (c0 + c < a.C) v[c].load(x + (c0 + c) * a.inner);
+  };
+  read(0);  // (on their way while what the pixels share is read)
   RowGrad r[P];
   int target[P];
 #pragma unroll
@@ -785,13 +801,10 @@ template <typename T, int P> __global__ void __launch_bounds__(128) log_probs_pl
     r[p] = row_grad(a, at + p, o, i + p);
     target[p] = r[p].target >= 0 && r[p].target < a.C ? (int)r[p].target : -1;
   }
-  for (int c0 = 0; c0 < a.C; c0 += kPlaneChannels) {
-    PixelVector<T, P> v[kPlaneChannels];
+  for (int c0 = 0; c0 < a.C; c0 += CHANNELS) {
+    if (c0 > 0) read(c0);
 #pragma unroll
-    for (int c = 0; c < kPlaneChannels; c++)
-      if (c0 + c < a.C) v[c].load(x + (c0 + c) * a.inner);
-#pragma unroll
-    for (int c = 0; c < kPlaneChannels; c++)
+    for (int c = 0; c < CHANNELS; c++)
       if (c0 + c < a.C) {
 #pragma unroll
         for (int p = 0; p < P; p++) {
