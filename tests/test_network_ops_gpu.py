@@ -210,7 +210,7 @@ LOGPROB_SHAPES = [  # (shape, dim, ks)
     ((1, 131072), -1, (8,)), ((2, 131075), -1, (4,)), ((1, 300001), -1, (5,)), ((600, 1500), -1, (2,)), ((300, 70), -1, (3,)),
     ((2, 3, 50), -1, (2,)), ((3001, 10), -1, (0, 3)), ((515, 64), -1, (0, 1)), ((260, 129), -1, (0,)), ((70, 1016), -1, (0, 9)), ((70, 1023), -1, (0,)), ((1, 13, 8, 16), 1, (0, 1, 4, 13)), ((2, 41, 11, 13), 1, (3, 20)), ((3, 2, 5), 1, (0, 2)), ((1, 150, 3, 64), 1, (8,)),
     ((1, 1, 4, 5), 1, (1,)), ((2, 300, 1, 7), 1, (9,)), ((4, 19, 64, 64), 1, (0, 5)), ((7, 3, 9), 0, (2,)), ((2, 1031, 2, 3), 1, (4,)),
-    ((1, 5, 70000), 1, (0, 2)),
+    ((1, 5, 70000), 1, (0, 2)), ((1, 65537, 4), 1, (3,)), ((2, 50, 3, 8), 1, (3, 8, 50)),
 ]
 
 
