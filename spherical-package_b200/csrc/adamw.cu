@@ -35,22 +35,11 @@ template <int CAP> struct AdamArgs {
   const float *lr_at, *step_at;
 };
 
-// A lane's eight neighbouring values, in loads and stores of up to 32 bytes.
-__device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
-  asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
-               : "l"(p));
-}
+// A lane's eight neighbouring values, in stores of up to 32 bytes.
 __device__ __forceinline__ void store8(float *p, const float (&v)[8]) {
   asm volatile("st.global.v8.f32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),
                "f"(v[5]), "f"(v[6]), "f"(v[7]), "l"(p)
                : "memory");
-}
-template <typename T> __device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
-  union { uint4 u; T t[8]; } q;
-  q.u = *(const uint4 *)p;
-#pragma unroll
-  for (int i = 0; i < 8; i++) v[i] = to_float(q.t[i]);
 }
 template <typename T> __device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
   union { uint4 u; T t[8]; } q;
@@ -63,15 +52,6 @@ struct E4m3 {
 };
 __device__ __forceinline__ float to_float(E4m3 v) { return from_e4m3(v.v); }
 template <> __device__ __forceinline__ E4m3 from_float<E4m3>(float v) { return E4m3{to_e4m3(v)}; }
-__device__ __forceinline__ void load8(const E4m3 *p, float (&v)[8]) {
-  const uint2 q = *(const uint2 *)p;
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const unsigned two = ((i < 2 ? q.x : q.y) >> (16 * (i & 1))) & 0xffffu;
-    const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3)));
-    v[2 * i] = f.x, v[2 * i + 1] = f.y;
-  }
-}
 __device__ __forceinline__ void store8(E4m3 *p, const float (&v)[8]) {
   unsigned q[4];
 #pragma unroll
@@ -79,7 +59,7 @@ __device__ __forceinline__ void store8(E4m3 *p, const float (&v)[8]) {
   *(uint2 *)p = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
 }
 
-// A lane's eight values as they are in memory.
+// The same values as they are in memory, in loads of up to 32 bytes.
 template <typename T> struct Raw {
   unsigned w[2 * sizeof(T)];
   __device__ __forceinline__ void load(const T *p) {

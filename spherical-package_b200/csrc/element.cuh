@@ -20,9 +20,6 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// What a value is once it has been stored as T.
-template <typename T> __device__ __forceinline__ float as_stored(float v) { return to_float(from_float<T>(v)); }
-
 // A weight of its own type, float32 or the data's.
 template <typename T> __device__ __forceinline__ float load_weight(const void *w, int64_t i, bool f32) {
   return f32 ? __ldg((const float *)w + i) : to_float(((const T *)w)[i]);
@@ -103,9 +100,6 @@ template <class F> __device__ __forceinline__ float block_join(float v, float *s
 // Asynchronous copies into shared memory.
 __device__ __forceinline__ void copy_16(void *to, const void *from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copy_8(void *to, const void *from) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copy_4(void *to, const void *from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
