@@ -133,15 +133,13 @@ __device__ __forceinline__ float largest_of(float (&v)[8]) {
   }
   return amax;
 }
-// Two scales at once: amax / 448 and 448 / amax of both are one division, in four lanes of four.
+// Both moments' scales; their reciprocals are one, in two lanes.
 struct Scales {
   float m, m_inverse, u, u_inverse;
   __device__ __forceinline__ Scales(float m_max, float u_max) {
-    const int lane = threadIdx.x & 31;
-    const float amax = lane & 2 ? u_max : m_max;
-    const float q = amax < kTiny ? 0.f : (lane & 1 ? kE4m3Max : amax) / (lane & 1 ? amax : kE4m3Max);
-    m = __shfl_sync(0xffffffffu, q, 0), m_inverse = __shfl_sync(0xffffffffu, q, 1);
-    u = __shfl_sync(0xffffffffu, q, 2), u_inverse = __shfl_sync(0xffffffffu, q, 3);
+    const Scale s = Scale::of(threadIdx.x & 1 ? u_max : m_max);
+    m = __shfl_sync(0xffffffffu, s.scale, 0), m_inverse = __shfl_sync(0xffffffffu, s.inverse, 0);
+    u = __shfl_sync(0xffffffffu, s.scale, 1), u_inverse = __shfl_sync(0xffffffffu, s.inverse, 1);
   }
 };
 
@@ -208,8 +206,8 @@ __global__ void __launch_bounds__(256, EIGHT ? 3 : 4) adamw_kernel(const __grid_
       }
     }
     if (EIGHT) fetch(j + 1);
-    // The old moment's product and the root are rounded by themselves, the new term is fused: codes are cut from these
-    // values, and would otherwise depend on what the compiler fuses.
+    // The old moment's product and the root are rounded by themselves, the new term is fused, as elementary tensor operations do
+    // it: codes are cut from these values, and would otherwise depend on what the compiler fuses.
     const auto two = [](float x) { return make_float2(x, x); };
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
@@ -221,7 +219,7 @@ __global__ void __launch_bounds__(256, EIGHT ? 3 : 4) adamw_kernel(const __grid_
       }
       gi = mul_pair(gi, two(a.grad_scale));
       mi = fma_pair(two(a.rest1), gi, mul_pair(two(a.beta1), mi));
-      vi = fma_pair(mul_pair(two(a.rest2), gi), gi, mul_pair(two(a.beta2), vi));
+      vi = fma_pair(two(a.rest2), mul_pair(gi, gi), mul_pair(two(a.beta2), vi));
       const float2 u = make_float2(sqrtf(vi.x), sqrtf(vi.y)), d = fma_pair(u, two(root), two(a.eps));
       const float2 q = make_float2(__fdividef(mi.x, d.x), __fdividef(mi.y, d.y));
       wi = fma_pair(two(-step_size), q, mul_pair(wi, two(keep)));

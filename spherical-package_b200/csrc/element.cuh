@@ -34,11 +34,12 @@ template <typename T> __device__ __forceinline__ void store_weight(void *w, int6
 // Values held in 8 bits: e4m3 times a float32 scale, the largest magnitude of a group at e4m3's largest, 448.  A group
 // whose values all lie below kTiny (448 / amax would not be finite much below it) is a group of zeros with scale 0.
 constexpr float kE4m3Max = 448.f, kTiny = 0x1p-100f;
+// (the reciprocals are rounded before they are multiplied, as elementary tensor operations do it)
 struct Scale {
   float scale, inverse;
   static __device__ __forceinline__ Scale of(float amax) {
     const bool zero = amax < kTiny;
-    return Scale{zero ? 0.f : amax / kE4m3Max, zero ? 0.f : kE4m3Max / amax};
+    return Scale{zero ? 0.f : amax * (1.f / kE4m3Max), zero ? 0.f : __fmul_rn(__frcp_rn(amax), kE4m3Max)};
   }
 };
 __device__ __forceinline__ __nv_fp8_storage_t to_e4m3(float v) { return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
