@@ -167,11 +167,14 @@ template <typename T, int V> struct Tile {
   }
   // f(order, index) for each logit of order `least` or better.
   template <class F> __device__ __forceinline__ void each(unsigned least, int at, int step, int end, int shift, int C, F f) const {
+    const float bound = value_of(least);
 #pragma unroll
     for (int i = 0; i < V; i++)
 #pragma unroll
       for (int j = 0; j < N; j++) {
-        const unsigned o = order_of(v[i].at(j));
+        const float value = v[i].at(j);
+        if (value < bound) continue;  // (a bound that is NaN lets all pass)
+        const unsigned o = order_of(value);
         const int index = (at + i * step) * N - shift + j;
         if (o >= least && at + i * step < end && index >= 0 && index < C) f(o, index);
       }
@@ -205,8 +208,8 @@ constexpr int kRowThreads = 256, kMostTop = 32, kMostCandidates = 1024, kMostClu
 // tiles held in registers, each read once, the next one while it works on one.  With TOP (k > 0) it finds the best of each tile
 // without looking at most of it: the k-th largest of the maxima of 32 groups of threads is a bound that k logits reach and few
 // others do.  The blocks of a cluster put what they found into the first one's shared memory.  A few rows are latency: 8 x 131072
-// float32 with the best eight take 8.9 us in clusters of 16 (5.1 without best; 15 where the first block fetched the others' lists one by
-// one, 287 by one block a row in nine passes).
+// float32 with the best eight take 7.7 us in clusters of 16 (4.2 without best; 15 where the first block fetched the others' lists one by
+// one, 287 by one block a row in nine passes); 1000 x 32000 49 us (2.6 TB/s), by the barriers and scans of each row's first tile.
 template <typename T, bool TOP> struct RowKernel {
   static constexpr int V = TOP ? 32 / RowVector<T>::N : 4, TILE = kRowThreads * V * RowVector<T>::N;  // logits of a tile
 };
@@ -229,6 +232,9 @@ template <typename T, bool TOP> __global__ void __launch_bounds__(kRowThreads, T
   int have = 0, now = 0;  // candidates kept so far, in best[now]
   Tile<T, V> tile;
   tile.load(x, from + threadIdx.x, kRowThreads, end, shift, a.C);
+  // (two loads behind one another that would otherwise wait at the end)
+  const int64_t target = threadIdx.x == 0 && part == 0 ? a.target[row] : -1;
+  const float x_t = target >= 0 && target < a.C ? to_float(x[target]) : 0.f;
   constexpr int STEP = kRowThreads * V;
   if (!TOP) {
     for (int v0 = from; v0 < end; v0 += 2 * STEP) {
@@ -242,17 +248,21 @@ template <typename T, bool TOP> __global__ void __launch_bounds__(kRowThreads, T
   for (int v0 = from; TOP && v0 < end; v0 += STEP) {
     const int at = v0 + threadIdx.x;
     const float largest = tile.largest();
-    {
-      const unsigned mine = order_of(largest);
-      unsigned o = mine;
+    // Once there are k, only what is better than the worst of them counts, and most tiles have nothing of that.
+    const unsigned mine = order_of(largest);
+    const bool full = have == a.k;
+    const Candidate worst = full ? best[now][a.k - 1] : 0;
+    if (!full || __syncthreads_or(mine >= (unsigned)(worst >> 32))) {
+      if (!full) {
+        unsigned o = mine;
 #pragma unroll
-      for (int d = 4; d > 0; d >>= 1) o = max(o, __shfl_xor_sync(0xffffffffu, o, d));
-      if ((lane & 7) == 0) group_best[threadIdx.x >> 3] = o;
+        for (int d = 4; d > 0; d >>= 1) o = max(o, __shfl_xor_sync(0xffffffffu, o, d));
+        if ((lane & 7) == 0) group_best[threadIdx.x >> 3] = o;
+      }
       if (threadIdx.x < have) pool[threadIdx.x] = best[now][threadIdx.x];
       if (threadIdx.x == 0) pooled = have;
       __syncthreads();
-      const Candidate worst = have == a.k ? best[now][a.k - 1] : 0;
-      const unsigned least = max(kth_largest(group_best[lane], a.k), (unsigned)(worst >> 32));
+      const unsigned least = full ? (unsigned)(worst >> 32) : kth_largest(group_best[lane], a.k);
       if (mine >= least)
         tile.each(least, at, kRowThreads, end, shift, a.C, [&](unsigned order, int index) {
           const Candidate c = candidate(order, index);
@@ -301,9 +311,10 @@ template <typename T, bool TOP> __global__ void __launch_bounds__(kRowThreads, T
   __syncthreads();
   if (blocks > 1) {
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every block has started, so its shared memory may be written
-    if (threadIdx.x == 0) {
-      for (int i = 1; i < 8; i++) st.join(Stats::of(stats[i]));
-      cluster.map_shared_rank(&parts[0], 0)[part] = st.packed();
+    if (warp == 0) {
+      st = Stats::of(stats[lane & 7]);
+      st.join_lanes(8);
+      if (lane == 0) cluster.map_shared_rank(&parts[0], 0)[part] = st.packed();
     }
     if (TOP && threadIdx.x < a.k)
       cluster.map_shared_rank(&gathered[0], 0)[part * a.k + threadIdx.x] = threadIdx.x < have ? best[now][threadIdx.x] : 0;
@@ -315,14 +326,14 @@ template <typename T, bool TOP> __global__ void __launch_bounds__(kRowThreads, T
       now ^= 1;
     }
   }
-  if (threadIdx.x == 0) {
+  if (warp == 0) {
     const int n = blocks > 1 ? blocks : 8;
-    const float4 *all = blocks > 1 ? parts : stats;
-    st = Stats::of(all[0]);
-    for (int i = 1; i < n; i++) st.join(Stats::of(all[i]));
-    whole = st.packed();
-    const int64_t t = a.target[row];
-    write_stats(a, row, st, t, t >= 0 && t < a.C ? to_float(x[t]) : 0.f);
+    st = lane < n ? Stats::of(blocks > 1 ? parts[lane] : stats[lane]) : Stats();
+    st.join_lanes(kMostCluster);
+    if (lane == 0) {
+      whole = st.packed();
+      write_stats(a, row, st, target, x_t);
+    }
   }
   if (!TOP) return;
   __syncthreads();
@@ -334,7 +345,7 @@ template <typename T, bool TOP> __global__ void __launch_bounds__(kRowThreads, T
 }
 
 // Many rows without best classes: the blocks walk over the rows, and their next tiles, of the next rows too, are on their way into
-// shared memory, where every thread reads what it has copied itself.  4096 x 32000 bf16 take 60 us (4.4 TB/s): 45 us of loads; of the
+// shared memory, where every thread reads what it has copied itself.  4096 x 32000 bf16 take 59 us (4.4 TB/s): 45 us of loads; of the
 // exponentials (131M at 16 a cycle of an SM are 29 us) and of issue not all hides behind them; with a block a row 66 us.
 constexpr int kRowStages = 3, kStreamThreads = 128, kStreamBlocks = 8;
 template <typename T> __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) log_probs_stream_kernel(LogProbArgs a) {
@@ -380,7 +391,15 @@ template <typename T> __global__ void __launch_bounds__(kStreamThreads, kStreamB
   for (int d = 0; d < kRowStages - 1; d++) copy(d);
   Stats st;
   int stage = 0, turn = 0;
+  // the row's target and its logit, the first fetched a row ahead
+  int64_t target = -1, target_next = threadIdx.x == 0 && here.row < a.outer ? a.target[here.row] : -1;
+  float x_t = 0.f;
   while (here.row < a.outer) {
+    if (threadIdx.x == 0 && here.v0 == 0) {
+      target = target_next;
+      x_t = target >= 0 && target < a.C ? to_float(here.x[target]) : 0.f;
+      if (here.row + gridDim.x < a.outer) target_next = a.target[here.row + gridDim.x];
+    }
     copy(stage == 0 ? kRowStages - 1 : stage - 1);
     copies_wait<kRowStages - 1>();
     Tile<T, V> tile;
@@ -396,7 +415,6 @@ template <typename T> __global__ void __launch_bounds__(kStreamThreads, kStreamB
     tile.add_to(st, tile.largest());
     stage = stage == kRowStages - 1 ? 0 : stage + 1;
     const int64_t row = here.row;
-    const T *x = here.x;
     here.next(a);
     if (here.row == row) continue;
     st.join_warp();
@@ -404,8 +422,7 @@ template <typename T> __global__ void __launch_bounds__(kStreamThreads, kStreamB
     __syncthreads();
     if (threadIdx.x == 0) {
       for (int i = 1; i < kStreamThreads / 32; i++) st.join(Stats::of(stats[turn][i]));
-      const int64_t t = a.target[row];
-      write_stats(a, row, st, t, t >= 0 && t < a.C ? to_float(x[t]) : 0.f);
+      write_stats(a, row, st, target, x_t);
     }
     st = Stats();
     turn ^= 1;

@@ -611,6 +611,36 @@ def test_training_step_in_two_graphs(capturable_bits):
     assert o.param_groups[0]["step"].item() == 5
 
 
+def test_forwards_replayed_with_new_inputs():
+    """Every forward kernel family in one graph, replayed on other values: what an eager call gives."""
+    rows = {n: normal((5, n), n) for n in (30, 1000, 5001, 40000)}
+    planes = {c: normal((2, c, 12, 20), c) for c in (5, 64, 300)}
+    odd = normal((2, 40, 33, 31), 7)
+    targets = {5: torch.zeros(5, dtype=torch.long, device="cuda"), (2, 12, 20): torch.zeros((2, 12, 20), dtype=torch.long, device="cuda")}
+
+    def everything():
+        out = []
+        for x in rows.values():
+            out += [*F.token_log_probs(x, targets[5], -1, 4), *F.token_log_probs(x, targets[5], -1)[:2]]
+            out += [F.rms_norm(x, None, None, EPS, -1), *F.rms_norm_quantized(x, None, x, EPS, -1)]
+        for x in planes.values():
+            out += [*F.token_log_probs(x, targets[2, 12, 20], 1, 2), F.rms_norm(x, None, x, EPS, 1)[0], *F.rms_norm_quantized(x, None, None, EPS, 1)]
+        return out + [F.rms_norm(odd, None, None, EPS, 1)]
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        everything()
+    torch.cuda.current_stream().wait_stream(st)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = everything()
+    for x in (*rows.values(), *planes.values(), odd):
+        x.copy_(torch.randn_like(x) * 2)
+    g.replay()
+    for a, b in zip(got, everything()):
+        assert torch.equal(a.float(), b.float())
+
+
 def test_mapped_network_step():
     """As they are used together: mapped convolution, norm with a skip connection, mapped head, labels of pixels, backward, AdamW;
     every gradient against the same network of plain operators."""
