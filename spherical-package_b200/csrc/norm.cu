@@ -142,19 +142,18 @@ template <typename T> __global__ void __launch_bounds__(256) norm_deep_planes_we
   if (threadIdx.x == 0) a.partial[(int64_t)blockIdx.y * a.C + c] = v;
 }
 
-// Sums of the partial weight gradients: 32 channels a block, eight threads over the splits of each.
-template <typename T> __global__ void __launch_bounds__(256) norm_weight_reduce_kernel(NormGradArgs a) {
-  __shared__ float shared[8][32];
+// Sums of the partial weight gradients: 32 channels a block, 32 threads over the splits of each.
+template <typename T> __global__ void __launch_bounds__(1024) norm_weight_reduce_kernel(NormGradArgs a) {
+  __shared__ float shared[32][33];
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float v = 0.f;
   if (c < a.C)
-    for (int i = part; i < a.splits; i += 8) v += a.partial[(int64_t)i * a.C + c];
+    for (int i = part; i < a.splits; i += 32) v += a.partial[(int64_t)i * a.C + c];
   shared[part][lane] = v;
   __syncthreads();
-  if (part == 0 && c < a.C) {
-    for (int i = 1; i < 8; i++) v += shared[i][lane];
-    store_weight<T>(a.gw, c, v, a.weight_f32);
-  }
+  v = warp_sum(shared[lane][part]);  // (a warp a channel)
+  const int mine = blockIdx.x * 32 + part;
+  if (lane == 0 && mine < a.C) store_weight<T>(a.gw, mine, v, a.weight_f32);
 }
 
 // ---- rows in registers -----------------------------------------------------------------------------------------------
@@ -235,8 +234,9 @@ template <bool WARP> __device__ __forceinline__ float row_sum(float v, float *sh
 // A row is held by a warp (WARP) or by a block, E elements a thread in pieces of N: every tensor is read and written once.
 // AHEAD: the blocks walk over the rows, and the next ones are on their way into shared memory, where every thread reads what it
 // has copied itself.  HBM bounds it: 8192 x 4096 bf16 with a residual take 45 us (5.9 TB/s; 50 without copying ahead), one row of 5120
-// to 8 bits 3 us, a launch and two barriers.
-constexpr int kRowStages = 3;
+// to 8 bits 3 us, a launch and two barriers.  More than one row ahead gains nothing (backward of the same: 50 us with two stages, 51 and
+// 53 with three and four; rows of 16384 133 us a pass and 174, whose third stage leaves no room for a second block).
+constexpr int kRowStages = 2;
 template <typename T, bool E4M3, int N, int E, bool WARP, bool AHEAD>
 __global__ void __launch_bounds__(WARP ? 256 : 512, AHEAD && E == 8 ? (WARP ? 4 : 2) : 1) norm_rows_kernel(NormArgs a) {
   constexpr int V = E / N;
@@ -337,8 +337,8 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, AHEAD && E == 8 ? (WARP ? 4 
 }
 
 // Backward: the blocks walk over the rows; a thread's channels stay the same, and their weights and weight gradients in its
-// registers, so that the weight gradient costs no second pass over both tensors.  8192 x 4096 bf16 with both output gradients: 52 us
-// (5.2 TB/s; 83 without copying ahead, between whose rows nothing was on its way).
+// registers, so that the weight gradient costs no second pass over both tensors.  8192 x 4096 bf16 with both output gradients: 50 us
+// (5.4 TB/s; 83 without copying ahead, between whose rows nothing was on its way).
 template <typename T, int N, int E, bool WARP, bool ADD, bool AHEAD>
 __global__ void __launch_bounds__(WARP ? 256 : 512, E == 8 ? (WARP ? 4 : 2) : 1) norm_rows_grad_kernel(NormGradArgs a) {
   constexpr int V = E / N, TENSORS = ADD ? 3 : 2;
@@ -566,7 +566,7 @@ template <typename T> int norm_grad_launch(NormGradArgs &a, int dtype, cudaStrea
     }
   }
   if (a.gw) {
-    norm_weight_reduce_kernel<T><<<(unsigned)cdiv(a.C, 32), 256, 0, st>>>(a);
+    norm_weight_reduce_kernel<T><<<(unsigned)cdiv(a.C, 32), 1024, 0, st>>>(a);
     launches++;
   }
   return launches;
