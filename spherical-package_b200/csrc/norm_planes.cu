@@ -5,7 +5,7 @@
 namespace sph {
 
 // HBM bounds it where planes are aligned: 16 x 256 x 128 x 256 float32 with a residual take 347 us (6.2 TB/s).  Odd planes are read
-// and written one pixel at a time behind the copies and are bound by issue: 3 x 96 x 181 x 333 bf16 to 8 bits 25 us (2.1 TB/s).
+// and written one pixel at a time behind the copies and are bound by issue: 3 x 96 x 181 x 333 bf16 to 8 bits 23 us (2.3 TB/s).
 template <typename T, bool E4M3, bool ADD, int MODE, int LOG, int U> __global__ void __launch_bounds__(kPlaneThreads, 4) norm_planes_kernel(NormArgs a, PlaneTile tile) {
   using L = Lane<T, MODE, LOG, U>;
   using G = Geometry<T, MODE, LOG, U>;

@@ -117,6 +117,29 @@ template <typename T, int MODE, int LOG, int U, class R> __device__ __forceinlin
     constexpr int PIECES = G::PIXELS / V + 1;  // a row's, from the boundary before it
     const T *base = from + run.offset(0), *last = from + run.total * run.C;
     const int count = (int)min((int64_t)G::PIXELS, run.inner - run.start);
+    if constexpr (LOG == 3) {  // a warp its own channels, whose shift is one
+      const int first = threadIdx.x >> 5, piece = threadIdx.x & 31, at = piece * V - shift_of(base, 0, first, run.inner);
+      // (all but the tensor's first and last pixels have something before and behind them)
+      const bool whole = base - V >= from && base + (run.C - 1) * run.inner + G::PIXELS + V <= last;
+      if (piece >= PIECES || at >= count) return;
+      const T *p = base + first * run.inner + at;
+      T *q = to + first * G::PITCH + piece * V;
+      const int64_t step = G::ACROSS * run.inner;
+      if (whole) {
+#pragma unroll 4
+        for (int c = first; c < run.C; c += G::ACROSS, p += step, q += G::ROW) copy_16(q, p);
+      } else {
+        for (int c = first; c < run.C; c += G::ACROSS, p += step, q += G::ROW) {
+          if (p >= from && p + V <= last) {
+            copy_16(q, p);
+          } else {
+            for (int e = 0; e < V; e++)
+              if (at + e >= 0 && at + e < count) q[e] = p[e];
+          }
+        }
+      }
+      return;
+    }
 #pragma unroll 4
     for (int i = threadIdx.x; i < run.C * PIECES; i += kPlaneThreads) {
       const int c = i / PIECES, j = i % PIECES, at = j * V - shift_of(base, 0, c, run.inner);
