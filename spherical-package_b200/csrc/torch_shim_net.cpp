@@ -89,17 +89,17 @@ std::vector<int64_t> sizes_without(const Tensor &t, int64_t dim) {
   s.erase(s.begin() + dim);
   return s;
 }
-// A dense tensor of the layout's order with n values along its dimension.
+// A dense tensor of the layout's order with n values along its dimension.  (Made with its strides, not as a view, which autograd
+// would not let be written in place.)
 Tensor like_layout(const Tensor &t, const Layout &l, int64_t n, torch::ScalarType type) {
-  std::vector<int64_t> s = t.sizes().vec();
+  std::vector<int64_t> s = t.sizes().vec(), strides(s.size(), 1);
   const auto options = t.options().dtype(type).memory_format(c10::nullopt).requires_grad(false);
-  if (!l.moved) {
-    s[l.dim] = n;
-    return torch::empty(s, options);
-  }
-  s = sizes_without(t, l.dim);
-  s.push_back(n);
-  return torch::empty(s, options).movedim(-1, l.dim);
+  s[l.dim] = n;
+  if (!l.moved) return torch::empty(s, options);
+  int64_t step = n;
+  for (int64_t i = t.dim() - 1; i >= 0; i--)
+    if (i != l.dim) strides[i] = step, step *= std::max<int64_t>(s[i], 1);
+  return torch::empty_strided(s, strides, options);
 }
 // Another tensor of the same sizes, dense in that order (copied if it is not).
 Tensor in_layout(const Tensor &t, const Layout &l) {

@@ -97,6 +97,22 @@ def test_norm_quantized(shape, dim, dtype):
     check_quantized(x, None, None, dim)
 
 
+def test_results_in_a_channels_last_layout_are_written_in_place():
+    """As contiguous ones are: an activation in place behind the norm, and its gradient, which is that of the one beside it."""
+    img = normal((2, 24, 5, 3), 3).contiguous(memory_format=torch.channels_last)
+    w, r = normal((24,), 4), normal((2, 24, 5, 3), 5).contiguous(memory_format=torch.channels_last)
+    grads = []
+    for relu in (torch.relu, torch.relu_):
+        leaf = [t.clone().requires_grad_() for t in (img, w, r)]
+        out, s = F.rms_norm(leaf[0], leaf[1], leaf[2], EPS, 1)
+        grads.append(torch.autograd.grad((relu(out) * 3).sum(), leaf))
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
+    top = F.token_log_probs(img.clone().requires_grad_(), torch.zeros((2, 5, 3), dtype=torch.int64, device="cuda"), top_k=2).top_log_probs
+    top.mul_(2)
+    top.sum().backward()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("c", [64, 65, 1000, 4096])
 def test_norm_of_wider_rows_and_channels_last(c, dtype):
