@@ -106,6 +106,32 @@ Tensor in_layout(const Tensor &t, const Layout &l) {
   return l.moved ? t.movedim(l.dim, -1).contiguous().movedim(-1, l.dim) : t.contiguous();
 }
 
+// What a node saves goes through whatever hooks are set (to the host and back, say), which may bring it back with other strides;
+// the kernels are given nothing that is not what was saved otherwise.
+void came_back(bool same) { TORCH_CHECK(same, "a saved tensor's hooks returned another size, dtype or device than was saved"); }
+Tensor came_back(const Tensor &t, int64_t numel, torch::ScalarType type, const Tensor &like) {
+  came_back(t.defined() && t.numel() == numel && t.scalar_type() == type && t.layout() == torch::kStrided && t.device() == like.device());
+  return t.contiguous();
+}
+// The input (or the sum) of a node: in the layout that it had, or dense in that order.
+struct SavedInput {
+  SavedVariable saved;
+  at::DimVector sizes, strides;
+  torch::ScalarType type;
+  c10::Device device = c10::kCPU;
+  void set(const Tensor &t, bool output) {
+    saved = SavedVariable(t, output);
+    sizes = at::DimVector(t.sizes()), strides = at::DimVector(t.strides()), type = t.scalar_type(), device = t.device();
+  }
+  // `l.stride` becomes that of what is returned.
+  Tensor unpack(std::shared_ptr<Node> node, Layout &l) const {
+    Tensor t = saved.unpack(std::move(node));
+    came_back(t.defined() && t.sizes() == at::IntArrayRef(sizes) && t.scalar_type() == type && t.layout() == torch::kStrided && t.device() == device);
+    if (t.strides() != at::IntArrayRef(strides)) t = in_layout(t, l), l.stride = l.C;
+    return t;
+  }
+};
+
 bool transformed(std::initializer_list<const Tensor *> ts) {
   if (at::tracer::impl::is_dispatch_enabled() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode))
     return true;
@@ -182,29 +208,33 @@ NormResult norm_forward(const Tensor &x, const Tensor &weight, const Tensor &res
 }
 
 struct RmsNormNode : public Node {
-  SavedVariable s, weight, rstd;
+  SavedInput s;
+  SavedVariable weight, rstd;
   bool added = false;  // s is the sum, an output
+  torch::ScalarType weight_type = torch::kFloat;
   Layout layout;
   std::mutex mu;
   std::string name() const override { return "RmsNormBackward"; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mu);
-    for (SavedVariable *v : {&s, &weight, &rstd}) v->reset_data();
+    for (SavedVariable *v : {&s.saved, &weight, &rstd}) v->reset_data();
   }
   variable_list apply(variable_list &&g) override {
     std::lock_guard<std::mutex> lock(mu);
     variable_list r(3);
     {
       at::NoGradGuard no_grad;
-      const Tensor x = added ? s.unpack(shared_from_this()) : s.unpack(), w = weight.unpack(), rs = rstd.unpack();
+      Layout l = layout;
+      const Tensor x = s.unpack(added ? shared_from_this() : nullptr, l), rs = came_back(rstd.unpack(), l.outer * l.inner, torch::kFloat, x);
+      Tensor w = weight.unpack();
+      if (w.defined()) w = came_back(w, l.C, weight_type, x);
       const bool want_x = task_should_compute_output(0) || task_should_compute_output(1), want_w = w.defined() && task_should_compute_output(2);
       Tensor gout = g[0], gsum = added && g.size() > 1 ? g[1] : Tensor();
       if (!gout.defined()) gout = torch::zeros_like(x);
       c10::cuda::CUDAGuard guard(x.device());
-      gout = in_layout(gout, layout);
-      if (gsum.defined()) gsum = in_layout(gsum, layout);
+      gout = in_layout(gout, l);
+      if (gsum.defined()) gsum = in_layout(gsum, l);
       const int dtype = element_of(x, "input");
-      const Layout &l = layout;
       Tensor gx, gw, ws;
       if (want_x) gx = like_layout(x, l, l.C, x.scalar_type());
       if (want_w) {
@@ -214,7 +244,7 @@ struct RmsNormNode : public Node {
       if (want_x || want_w)
         ok(sph_rms_norm_backward(gout.data_ptr(), gsum.defined() ? gsum.data_ptr() : nullptr, x.data_ptr(), w.defined() ? w.data_ptr() : nullptr,
                                  rs.data_ptr<float>(), want_x ? gx.data_ptr() : nullptr, want_w ? gw.data_ptr() : nullptr, l.outer, l.C,
-                                 l.inner, added ? l.C : l.stride, dtype,
+                                 l.inner, l.stride, dtype,
                                  w.defined() && w.scalar_type() == torch::kFloat ? SPH_F32 : dtype, want_w ? ws.data_ptr() : nullptr,
                                  want_w ? (size_t)ws.numel() : 0, current_stream()),
            "sph_rms_norm_backward");
@@ -244,7 +274,9 @@ c10::optional<std::vector<Tensor>> rms_norm(const Tensor &x, const OptTensor &we
     n->layout = r.layout;
     n->added = res.defined();
     torch::autograd::set_history(out, n);
-    n->s = n->added ? SavedVariable(out[1], true) : SavedVariable(x, false);
+    if (n->added) n->layout.stride = r.layout.C;  // (the sum is dense)
+    n->s.set(n->added ? out[1] : x, n->added);
+    if (w.defined()) n->weight_type = w.scalar_type();
     n->weight = SavedVariable(w, false);
     n->rstd = SavedVariable(r.rstd, false);
   }
@@ -261,14 +293,15 @@ std::vector<Tensor> rms_norm_quantized(const Tensor &x, const OptTensor &weight,
 
 // ---- log probabilities -----------------------------------------------------------------------------------------------
 struct LogProbsNode : public Node {
-  SavedVariable x, target, stats, entropy, top_index;
+  SavedInput x;
+  SavedVariable target, stats, entropy, top_index;
   Layout layout;
   int64_t k = 0, ignore_index = 0;
   std::mutex mu;
   std::string name() const override { return "TokenLogProbsBackward"; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mu);
-    for (SavedVariable *v : {&x, &target, &stats, &entropy, &top_index}) v->reset_data();
+    for (SavedVariable *v : {&x.saved, &target, &stats, &entropy, &top_index}) v->reset_data();
   }
   // One value for all (the gradient of a sum or a mean) is taken as such.
   static const float *spread(Tensor &g, int64_t &stride) {
@@ -287,15 +320,22 @@ struct LogProbsNode : public Node {
     variable_list r(1);
     {
       at::NoGradGuard no_grad;
-      const Tensor in = x.unpack(), t = target.unpack(), s = stats.unpack(), e = entropy.unpack(shared_from_this()), index = top_index.unpack();
       if (!task_should_compute_output(0)) return r;
-      const Layout &l = layout;
+      Layout l = layout;
+      const int64_t n = l.outer * l.inner;
+      const Tensor in = x.unpack(nullptr, l), t = came_back(target.unpack(), n, torch::kLong, in), s = came_back(stats.unpack(), 2 * n, torch::kFloat, in),
+                   e = came_back(entropy.unpack(shared_from_this()), n, torch::kFloat, in);
+      Tensor index = top_index.unpack();
       c10::cuda::CUDAGuard guard(in.device());
       r[0] = like_layout(in, l, l.C, in.scalar_type());
       int64_t g_stride, h_stride;
       const float *gp = spread(g[0], g_stride), *hp = spread(g[1], h_stride);
       Tensor gt = k > 0 && g.size() > 2 ? g[2] : Tensor();
-      if (gt.defined()) gt = in_layout(gt, l);
+      if (gt.defined()) {
+        gt = in_layout(gt, l);
+        came_back(index.defined() && index.sizes() == gt.sizes() && index.scalar_type() == torch::kLong && index.device() == in.device());
+        index = in_layout(index, l);
+      }
       ok(sph_token_log_probs_backward(in.data_ptr(), t.data_ptr<int64_t>(), s.data_ptr<float>(), e.data_ptr<float>(),
                                       gt.defined() ? index.data_ptr<int64_t>() : nullptr, gp, g_stride, hp, h_stride,
                                       gt.defined() ? gt.data_ptr<float>() : nullptr, r[0].data_ptr(), l.outer, l.C, l.inner, l.stride, k,
@@ -343,7 +383,7 @@ c10::optional<std::vector<Tensor>> token_log_probs(const Tensor &x, const Tensor
     n->k = k;
     n->ignore_index = ignore_index;
     torch::autograd::set_history(out, n);
-    n->x = SavedVariable(x, false);
+    n->x.set(x, false);
     n->target = SavedVariable(target, false);
     n->stats = SavedVariable(stats, false);
     n->entropy = SavedVariable(out[1], true);

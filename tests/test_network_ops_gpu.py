@@ -113,6 +113,37 @@ def test_results_in_a_channels_last_layout_are_written_in_place():
     top.sum().backward()
 
 
+def saved_cases():
+    """(input, dim): rows of wider rows, a channels-last image, planes."""
+    return [(normal((40, 72), 6)[:, 3:60], 1), (normal((2, 24, 5, 3), 7).contiguous(memory_format=torch.channels_last), 1),
+            (normal((2, 24, 5, 3), 8), 1), (normal((64, 4096), 9)[:, :2048], 1)]
+
+
+@pytest.mark.parametrize("pinned", [False, True])
+@pytest.mark.parametrize("case", range(4))
+def test_saved_tensors_may_come_back_with_other_strides(case, pinned):
+    """What a node saved is kept on the host until the backward pass, from where slices and channels-last images may come
+    back dense in another order."""
+    x, dim = saved_cases()[case]
+    w, target = normal((x.shape[dim],), 10), torch.zeros([s for i, s in enumerate(x.shape) if i != dim], dtype=torch.int64, device="cuda")
+    gout, gsum = normal(x.shape, 13), normal(x.shape, 14)
+    with torch.autograd.graph.save_on_cpu(pin_memory=pinned):
+        check_norm(x, w, None, dim, gout, None)
+        check_norm(x, w, x, dim, gout, gsum)
+        check_log_probs(x, target, dim, 3)
+
+
+@pytest.mark.parametrize("other", [lambda t: t.double(), lambda t: t.reshape(-1)[:1], lambda t: t.cpu()])
+def test_saved_tensors_that_come_back_as_others_are_refused(other):
+    x, w = normal((8, 96), 11).requires_grad_(), normal((96,), 12).requires_grad_()
+    target = torch.zeros(8, dtype=torch.int64, device="cuda")
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, other):
+        out, p = F.rms_norm(x, w, dim=1), F.token_log_probs(x, target, top_k=2)
+    for o in (out, p.log_probs, p.top_log_probs):
+        with pytest.raises(RuntimeError, match="hooks returned another"):
+            o.sum().backward(retain_graph=True)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("c", [64, 65, 1000, 4096])
 def test_norm_of_wider_rows_and_channels_last(c, dtype):
