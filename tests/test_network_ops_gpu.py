@@ -133,6 +133,65 @@ def test_saved_tensors_may_come_back_with_other_strides(case, pinned):
         check_log_probs(x, target, dim, 3)
 
 
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_recomputed_in_the_backward_pass(reentrant):
+    """Norms and log probabilities in a checkpointed block, whose forward pass runs again in the backward pass."""
+    from torch.utils.checkpoint import checkpoint
+    x, w = normal((2, 24, 5, 3), 15), normal((24,), 16)
+    target = torch.randint(24, (2, 5, 3), generator=gen(17), device="cuda")
+
+    def block(x, w):
+        out, s = F.rms_norm(x, w, x * 0.5, EPS, 1)
+        out = F.rms_norm(torch.relu_(out) + s, w, dim=1)
+        p = F.token_log_probs(out, target, top_k=2)
+        return p.log_probs.mean() + p.entropy.mean() + p.top_log_probs.mean()
+
+    grads = []
+    for kept in (True, False):
+        leaf = [x.clone().requires_grad_(), w.clone().requires_grad_()]
+        loss = block(*leaf) if kept else checkpoint(block, *leaf, use_reentrant=reentrant)
+        loss.backward()
+        grads.append([t.grad for t in leaf])
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
+
+
+def test_calls_from_two_threads():
+    """Each on its own stream, forward and backward; the same results as alone."""
+    import threading
+    xs, w = [normal((300, 512), 18), normal((64, 40, 9, 7), 19)], [normal((512,), 20), normal((40,), 21)]
+
+    def run(i):
+        leaf = [xs[i].clone().requires_grad_(), w[i].clone().requires_grad_()]
+        out = F.rms_norm(leaf[0], leaf[1], dim=1)
+        target = torch.zeros([s for d, s in enumerate(xs[i].shape) if d != 1], dtype=torch.int64, device="cuda")
+        p = F.token_log_probs(out, target, top_k=2)
+        return [out, p.log_probs, p.top_indices, *torch.autograd.grad(p.log_probs.sum() + p.entropy.sum(), leaf)]
+
+    alone, together, errors = [run(0), run(1)], [[], []], []
+    torch.cuda.synchronize()
+
+    def worker(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    together[i] = run(i)
+            stream.synchronize()
+        except Exception as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=worker, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for got, want in zip(together, alone):
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("other", [lambda t: t.double(), lambda t: t.reshape(-1)[:1], lambda t: t.cpu()])
 def test_saved_tensors_that_come_back_as_others_are_refused(other):
     x, w = normal((8, 96), 11).requires_grad_(), normal((96,), 12).requires_grad_()
