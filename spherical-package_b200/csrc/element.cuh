@@ -41,6 +41,12 @@ struct Scale {
     const bool zero = amax < kTiny;
     return Scale{zero ? 0.f : amax * (1.f / kE4m3Max), zero ? 0.f : __fmul_rn(__frcp_rn(amax), kE4m3Max)};
   }
+  // Of values p rstd, most = max |p|: the codes are p `inverse`, without rstd, whose last bit depends on the order in which a
+  // kernel has summed; so a norm's codes are the same from every kernel.
+  static __device__ __forceinline__ Scale of(float most, float rstd) {
+    const Scale r = of(most * rstd);
+    return Scale{r.scale, r.inverse > 0.f ? __fmul_rn(__frcp_rn(most), kE4m3Max) : r.inverse};
+  }
 };
 __device__ __forceinline__ __nv_fp8_storage_t to_e4m3(float v) { return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
 __device__ __forceinline__ float from_e4m3(__nv_fp8_storage_t v) {

@@ -26,19 +26,19 @@ template <typename T, bool E4M3> __global__ void __launch_bounds__(256) norm_lon
   const T *s = r ? sum : x;
   Scale sc{1.f, 1.f};
   if (E4M3) {
-    float amax = 0.f;
+    float most = 0.f;
     for (int c = threadIdx.x; c < a.C; c += 256)
-      amax = max_nan(amax, fabsf(to_float(s[c]) * rstd * (a.weight ? load_weight<T>(a.weight, c, a.weight_f32) : 1.f)));
-    amax = block_join(amax, shared, [](float p, float q) { return max_nan(p, q); });
-    sc = Scale::of(amax);
+      most = max_nan(most, fabsf(to_float(s[c]) * (a.weight ? load_weight<T>(a.weight, c, a.weight_f32) : 1.f)));
+    most = block_join(most, shared, [](float p, float q) { return max_nan(p, q); });
+    sc = Scale::of(most, rstd);
     if (threadIdx.x == 0) a.scale[row] = sc.scale;
   }
   for (int c = threadIdx.x; c < a.C; c += 256) {
-    const float y = to_float(s[c]) * rstd * (a.weight ? load_weight<T>(a.weight, c, a.weight_f32) : 1.f);
+    const float v = to_float(s[c]), w = a.weight ? load_weight<T>(a.weight, c, a.weight_f32) : 1.f;
     if (E4M3)
-      ((__nv_fp8_storage_t *)a.out)[row * a.C + c] = to_e4m3(y * sc.inverse);
+      ((__nv_fp8_storage_t *)a.out)[row * a.C + c] = to_e4m3(v * w * sc.inverse);
     else
-      ((T *)a.out)[row * a.C + c] = from_float<T>(y);
+      ((T *)a.out)[row * a.C + c] = from_float<T>(v * rstd * w);
   }
 }
 
@@ -64,18 +64,18 @@ template <typename T, bool E4M3> __global__ void __launch_bounds__(256) norm_dee
   const T *s = r ? sum : x;
   Scale sc{1.f, 1.f};
   if (E4M3) {
-    float amax = 0.f;
+    float most = 0.f;
     for (int c = 0; c < a.C; c++)
-      amax = max_nan(amax, fabsf(to_float(s[c * a.inner]) * rstd * (a.weight ? load_weight<T>(a.weight, c, a.weight_f32) : 1.f)));
-    sc = Scale::of(amax);
+      most = max_nan(most, fabsf(to_float(s[c * a.inner]) * (a.weight ? load_weight<T>(a.weight, c, a.weight_f32) : 1.f)));
+    sc = Scale::of(most, rstd);
     a.scale[at] = sc.scale;
   }
   for (int c = 0; c < a.C; c++) {
-    const float y = to_float(s[c * a.inner]) * rstd * (a.weight ? load_weight<T>(a.weight, c, a.weight_f32) : 1.f);
+    const float v = to_float(s[c * a.inner]), w = a.weight ? load_weight<T>(a.weight, c, a.weight_f32) : 1.f;
     if (E4M3)
-      ((__nv_fp8_storage_t *)a.out)[base + c * a.inner] = to_e4m3(y * sc.inverse);
+      ((__nv_fp8_storage_t *)a.out)[base + c * a.inner] = to_e4m3(v * w * sc.inverse);
     else
-      ((T *)a.out)[base + c * a.inner] = from_float<T>(y);
+      ((T *)a.out)[base + c * a.inner] = from_float<T>(v * rstd * w);
   }
 }
 
@@ -307,13 +307,13 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, AHEAD && E == 8 ? (WARP ? 4 
     }
     const float rstd = 1.f / sqrtf(row_sum<WARP>(sq, shared[turn][0], threads) * a.inv_c + a.eps);
     if (thread == 0 && a.rstd && C) a.rstd[row] = rstd;
-    float factor = rstd;
+    float inverse = 0.f;  // (E4M3)
     if (E4M3) {
       if (!WARP)
         most = warp_join(lane < (int)(blockDim.x >> 5) ? shared[turn][1][lane] : 0.f, [](float p, float q) { return max_nan(p, q); });
-      const Scale sc = Scale::of(most * rstd);
+      const Scale sc = Scale::of(most, rstd);
       if (thread == 0 && C) a.scale[row] = sc.scale;
-      factor *= sc.inverse;
+      inverse = sc.inverse;
     }
 #pragma unroll
     for (int i = 0; i < V; i++) {
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, AHEAD && E == 8 ? (WARP ? 4 
         float y[N];
         load_weights<T, N>(a.weight, c, a.weight_f32, y);
 #pragma unroll
-        for (int j = 0; j < N; j++) y[j] = to_float(s[i].t[j]) * factor * y[j];
+        for (int j = 0; j < N; j++) y[j] = E4M3 ? to_float(s[i].t[j]) * y[j] * inverse : to_float(s[i].t[j]) * rstd * y[j];
         if (E4M3) {
           store_e4m3<N>((__nv_fp8_storage_t *)a.out + row * a.C + c, y);
         } else {

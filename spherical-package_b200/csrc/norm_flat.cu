@@ -112,18 +112,18 @@ template <typename T, bool E4M3, bool ADD, int E, bool BLOCK> __global__ void __
       if (E4M3) most = warp_join(has ? shared[turn][1][lane] : 0.f, larger);
     }
     const float rstd = 1.f / sqrtf(sq * a.inv_c + a.eps);
-    float factor = rstd;
+    float inverse = 0.f;  // (E4M3)
     if (on && thread == 0 && a.rstd) a.rstd[row0 + i] = rstd;
     if (E4M3) {
-      const Scale sc = Scale::of(most * rstd);
+      const Scale sc = Scale::of(most, rstd);
       if (on && thread == 0) a.scale[row0 + i] = sc.scale;
-      factor *= sc.inverse;
+      inverse = sc.inverse;
     }
     T *out = ADD ? r + (at - x) : at;
 #pragma unroll
     for (int j = 0; j < E; j++)
       if (thread + j * threads < a.C && on) {
-        const float y = v[j] * factor * w(j);
+        const float y = E4M3 ? v[j] * w(j) * inverse : v[j] * rstd * w(j);
         if (E4M3)
           q[q_shift + i * a.C + thread + j * threads] = to_e4m3(y);
         else

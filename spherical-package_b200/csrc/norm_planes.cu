@@ -51,15 +51,15 @@ template <typename T, bool E4M3, bool ADD, int MODE, int LOG, int U> __global__ 
   }
   plane_join<LOG>(v, shared[0], [](float p, float q) { return p + q; });
   if (E4M3) plane_join<LOG>(most, shared[1], [](float p, float q) { return max_nan(p, q); });
-  float rstd[N], scale[N];
+  float rstd[N], inverse[N];
 #pragma unroll
   for (int i = 0; i < N; i++) {
     rstd[i] = 1.f / sqrtf(v[i] * a.inv_c + a.eps);
     if (first == 0 && px.in[i] && a.rstd) a.rstd[px.norm[i]] = rstd[i];
     if (E4M3) {
-      const Scale sc = Scale::of(most[i] * rstd[i]);
+      const Scale sc = Scale::of(most[i], rstd[i]);
       if (first == 0 && px.in[i]) a.scale[px.norm[i]] = sc.scale;
-      scale[i] = rstd[i] * sc.inverse;
+      inverse[i] = sc.inverse;
     }
   }
   plane = 0;
@@ -68,7 +68,7 @@ template <typename T, bool E4M3, bool ADD, int MODE, int LOG, int U> __global__ 
     typename L::P q = L::load(mine(k));
     float y[N];
 #pragma unroll
-    for (int i = 0; i < N; i++) y[i] = to_float(q.t[i]) * (E4M3 ? scale[i] : rstd[i]) * w[k * ACROSS];
+    for (int i = 0; i < N; i++) y[i] = E4M3 ? to_float(q.t[i]) * w[k * ACROSS] * inverse[i] : to_float(q.t[i]) * rstd[i] * w[k * ACROSS];
     if (E4M3) {
       px.store_e4m3((__nv_fp8_storage_t *)a.out, plane, y);
     } else {
