@@ -283,11 +283,15 @@ c10::optional<std::vector<Tensor>> rms_norm(const Tensor &x, const OptTensor &we
   return out;
 }
 
-std::vector<Tensor> rms_norm_quantized(const Tensor &x, const OptTensor &weight, const OptTensor &residual, double eps, int64_t dim) {
+// (out, scale) or (out, scale, sum), none with a gradient; nothing where what looks at the call would see the allocations alone.
+c10::optional<std::vector<Tensor>> rms_norm_quantized(const Tensor &x, const OptTensor &weight, const OptTensor &residual, double eps,
+                                                      int64_t dim, bool inside) {
+  const Tensor w = weight.value_or(Tensor()), res = residual.value_or(Tensor());
+  if (!inside && transformed({&x, &w, &res})) return c10::nullopt;
   at::NoGradGuard no_grad;
-  NormResult r = norm_forward(x, weight.value_or(Tensor()), residual.value_or(Tensor()), eps, dim, true, false);
+  NormResult r = norm_forward(x, w, res, eps, dim, true, false);
   std::vector<Tensor> out{r.out, r.scale};
-  if (residual) out.push_back(r.sum);
+  if (res.defined()) out.push_back(r.sum);
   return out;
 }
 
@@ -521,7 +525,8 @@ void adamw_step(const py::object &params_list, const py::object &grads_list, con
 void bind_network_ops(pybind11::module_ &m) {
   m.def("rms_norm_op", &rms_norm, py::arg("x"), py::arg("weight"), py::arg("residual"), py::arg("eps"), py::arg("dim"),
         py::arg("inside") = false);
-  m.def("rms_norm_quantized", &rms_norm_quantized, py::arg("x"), py::arg("weight"), py::arg("residual"), py::arg("eps"), py::arg("dim"));
+  m.def("rms_norm_quantized", &rms_norm_quantized, py::arg("x"), py::arg("weight"), py::arg("residual"), py::arg("eps"), py::arg("dim"),
+        py::arg("inside") = false);
   m.def("token_log_probs_op", &token_log_probs, py::arg("x"), py::arg("target"), py::arg("dim"), py::arg("top_k"),
         py::arg("ignore_index"), py::arg("inside") = false);
   m.def("adamw_step", &adamw_step, py::arg("params"), py::arg("grads"), py::arg("exp_avgs"), py::arg("exp_avg_sqs"), py::arg("masters"),

@@ -45,7 +45,7 @@ class _AsFunction(torch.autograd.Function):
         outs = out if many else (out,)
         ctx.wanted, ctx.inputs, ctx.outputs = wanted, [inner[i] for i in wanted], outs
         result = [o.detach() for o in outs]
-        ctx.mark_non_differentiable(*[o for o in result if not o.is_floating_point()])
+        ctx.mark_non_differentiable(*[r for o, r in zip(outs, result) if not o.requires_grad])
         return tuple(result) if many else result[0]
 
     @staticmethod
@@ -298,7 +298,11 @@ def rms_norm_quantized(input, weight=None, residual=None, eps=1e-6, dim=1):
     """rms_norm with its output in 8 bits: (q, scale), or (q, scale, s) with a residual, where q is float8_e4m3fn and
     q * scale.unsqueeze(dim) the output; scale (float32, the input's size without dim) is the largest magnitude of each
     normalised row / 448, and 0 over a row of zeros.  Forward only (no autograd node)."""
-    return tuple(_C.rms_norm_quantized(input, weight, residual, float(eps), int(dim)))
+    args = (input, weight, residual, float(eps), int(dim))
+    out = _C.rms_norm_quantized(*args)
+    if out is None:
+        out = _by_function(_C.rms_norm_quantized, args)
+    return tuple(out)
 
 
 class TokenLogProbs(NamedTuple):
