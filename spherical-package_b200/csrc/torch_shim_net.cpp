@@ -428,6 +428,7 @@ void adamw_step(const py::object &params_list, const py::object &grads_list, con
                 const py::object &masters_list, const py::object &m_scales_list, const py::object &v_scales_list, double step, double lr,
                 double beta1, double beta2, double eps, double weight_decay, double grad_scale, const OptTensor &step_at,
                 const OptTensor &lr_at) {
+  TORCH_CHECK(!at::tracer::impl::is_dispatch_enabled(), "adamw_step cannot be traced: a trace would hold nothing of it");
   const TensorList params(params_list, "param"), grads(grads_list, "grad"), m(m_list, "exp_avg"), v(v_list, "exp_avg_sq"),
       masters(masters_list, "master"), m_scales(m_scales_list, "exp_avg_scale"), v_scales(v_scales_list, "exp_avg_sq_scale");
   const size_t n = params.size();
