@@ -555,7 +555,8 @@ int sph_token_log_probs_backward(const void *x, const int64_t *target, const flo
  * each); v is held as its square root.  A block of 256 whose values are all
  * below 2^-100 is held as zeros.  step_at (DEVICE, may be NULL): the step's
  * number, instead of `step`, and lr_at then, if not NULL, instead of `lr`:
- * for steps that a CUDA graph replays.
+ * for steps that a CUDA graph replays.  What is written must not overlap
+ * anything else (not checked here).
  * ---------------------------------------------------------------------- */
 int sph_adamw_step(int64_t tensors, void *const *params, const void *const *grads, float *const *masters,
                    void *const *m, void *const *v, float *const *m_scales, float *const *v_scales,

@@ -40,6 +40,8 @@ int element_of(const Tensor &t, const char *name) {
   }
 }
 
+size_t element_bytes(int dtype) { return dtype == SPH_F32 ? 4 : 2; }
+
 void check_device(const Tensor &t, const char *name, const Tensor &like) {
   TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor (this build has no CPU path)");
   TORCH_CHECK(t.device() == like.device(), name, " must be on the same device as the input");
@@ -424,6 +426,41 @@ class TensorList {
   size_t size_ = 0;
 };
 
+// Whether a step's tensors lie apart in memory.  Those of a list mostly lie one behind the other and the lists apart: then nothing
+// has to be sorted.
+struct Span {
+  uintptr_t from = 0, to = 0;
+  bool written = true;
+};
+struct InOrder {
+  Span list[7];
+  bool so = true;
+  void next(int k, const void *p, size_t bytes) {
+    if (bytes == 0) return;
+    Span &l = list[k];
+    if (l.from == l.to) l.from = (uintptr_t)p;
+    so = so && (uintptr_t)p >= l.to;
+    l.to = (uintptr_t)p + bytes;
+  }
+  bool apart() const {
+    for (int i = 1; so && i < 7; i++)
+      for (int j = 0; j < i; j++)
+        if (list[i].from < list[j].to && list[j].from < list[i].to) return false;
+    return so;
+  }
+};
+// The same of any spans: nothing that is written shares memory with anything else.
+bool apart(std::vector<Span> spans) {
+  std::sort(spans.begin(), spans.end(), [](const Span &a, const Span &b) { return a.from < b.from; });
+  uintptr_t written = 0, read = 0;  // ends of what came so far
+  for (const Span &s : spans) {
+    if (s.from < written || (s.written && s.from < read)) return false;
+    uintptr_t &end = s.written ? written : read;
+    end = std::max(end, s.to);
+  }
+  return true;
+}
+
 void adamw_step(const py::object &params_list, const py::object &grads_list, const py::object &m_list, const py::object &v_list,
                 const py::object &masters_list, const py::object &m_scales_list, const py::object &v_scales_list, double step, double lr,
                 double beta1, double beta2, double eps, double weight_decay, double grad_scale, const OptTensor &step_at,
@@ -453,8 +490,7 @@ void adamw_step(const py::object &params_list, const py::object &grads_list, con
     std::vector<int64_t> n;
   };
   std::vector<Group> groups;
-  std::vector<const void *> seen;
-  seen.reserve(n);
+  InOrder order;
   const auto fits = [&](const Tensor &t, const char *name, torch::ScalarType type, int64_t numel) -> void * {
     TORCH_CHECK(t.scalar_type() == type, name, " must be ", type, ", got ", t.scalar_type());
     TORCH_CHECK(t.layout() == torch::kStrided && t.is_contiguous(), name, " must be contiguous");
@@ -485,12 +521,18 @@ void adamw_step(const py::object &params_list, const py::object &grads_list, con
     q.m.push_back(fits(m[i], "exp_avg", state, numel));
     q.v.push_back(fits(v[i], "exp_avg_sq", state, numel));
     q.n.push_back(numel);
-    if (master) q.w.push_back((float *)fits(masters[i], "master", torch::kFloat, numel));
+    const size_t state_bytes = eight ? numel : 4 * numel;
+    order.next(0, q.p.back(), element_bytes(dtype) * numel);
+    order.next(1, q.g.back(), element_bytes(grad_dtype) * numel);
+    order.next(2, q.m.back(), state_bytes);
+    order.next(3, q.v.back(), state_bytes);
+    if (master) q.w.push_back((float *)fits(masters[i], "master", torch::kFloat, numel)), order.next(4, q.w.back(), 4 * numel);
     if (eight) {
       q.ms.push_back((float *)fits(m_scales[i], "exp_avg_scale", torch::kFloat, blocks));
       q.vs.push_back((float *)fits(v_scales[i], "exp_avg_sq_scale", torch::kFloat, blocks));
+      order.next(5, q.ms.back(), 4 * blocks);
+      order.next(6, q.vs.back(), 4 * blocks);
     }
-    if (numel > 0) seen.push_back(q.p.back());
   }
   const auto scalar = [&](const OptTensor &t, const char *name) -> const float * {
     if (!t) return nullptr;
@@ -501,14 +543,22 @@ void adamw_step(const py::object &params_list, const py::object &grads_list, con
   const float *step_p = scalar(step_at, "step"), *lr_p = scalar(lr_at, "lr");
   const c10::Device device = like.device();
   const TensorList *lists[] = {&params, &grads, &m, &v, &masters, &m_scales, &v_scales};
+  if (!order.apart()) {
+    std::vector<Span> spans;
+    for (const TensorList *list : lists)
+      for (size_t i = 0; *list && i < n; i++)
+        if (list->has(i) && (*list)[i].numel() > 0) {
+          const uintptr_t from = (uintptr_t)(*list)[i].unsafeGetTensorImpl()->data();
+          spans.push_back({from, from + (*list)[i].nbytes(), list != &grads});
+        }
+    TORCH_CHECK(apart(std::move(spans)), "adamw_step: a tensor that is written appears twice, or overlaps another");
+  }
   for (const TensorList *list : lists)
     for (size_t i = 0; *list && i < n; i++)
       if (list->has(i)) {
         const Tensor &t = (*list)[i];
         TORCH_CHECK(t.is_cuda() && t.device() == device, "every tensor of adamw_step must be a CUDA tensor of one device (this build has no CPU path)");
       }
-  std::sort(seen.begin(), seen.end());
-  TORCH_CHECK(std::adjacent_find(seen.begin(), seen.end()) == seen.end(), "adamw_step: a param appears twice");
   c10::cuda::CUDAGuard guard(device);
   for (Group &q : groups)
     ok(sph_adamw_step((int64_t)q.n.size(), q.p.data(), q.g.data(), q.master ? q.w.data() : nullptr, q.m.data(), q.v.data(),
