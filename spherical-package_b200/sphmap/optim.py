@@ -19,8 +19,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.
     params float32, bfloat16 or float16, CUDA and contiguous like everything else here; grads of their params' dtype or
     float32.  masters: float32 copies of 16-bit params (None for any other), which are then what is updated, the param being
     its rounding.  exp_avgs and exp_avg_sqs (m, v): float32, or, with scales, float8_e4m3fn with a float32 scale for each 256
-    values, ceil(numel / 256) for a tensor; v is then held as its square root.  What is written must not overlap anything else.  step: the number of this step, from 1, or a
-    float32 CUDA tensor that holds it, for CUDA graphs; lr may be a tensor too then."""
+    values, ceil(numel / 256) for a tensor; v is then held as its square root.  What is written must not overlap anything else.
+    step: the number of this step, from 1, or a float32 CUDA tensor that holds it, for CUDA graphs; lr may be a tensor too then."""
     on_device = isinstance(step, torch.Tensor)
     lr_at = lr if isinstance(lr, torch.Tensor) else None
     _C.adamw_step(params, grads, exp_avgs, exp_avg_sqs, masters, exp_avg_scales, exp_avg_sq_scales, 0.0 if on_device else float(step),

@@ -106,7 +106,8 @@ class EncoderStack:
     convolution kernels (sph_mapped_conv_relu_*); without it as separate passes over the activations, the way the
     reference's operators compose.  With `optimizer`, which makes a torch optimizer from the list of parameters (such as
     `lambda p: sphmap.optim.AdamW(p, lr=1e-3)`), every step ends with an update of the weights and biases from the gradients
-    that the ranks have exchanged."""
+    that the ranks have exchanged.  What it updates are copies of the config's (`parameters()`); without an optimizer the stack reads the
+    config's own, where they lie on the device already."""
 
     def __init__(self, cfg, device, precision, local_batch, reducer=None, timers=None, fuse_relu=True, companions=None, optimizer=None):
         from . import capi
@@ -116,8 +117,10 @@ class EncoderStack:
         self.layers = cfg["layers"]
         self.dev = device
         self.B = local_batch
-        self.w = [t.to(device) for t in cfg["weights"]]
-        self.b = [t.to(device) for t in cfg["biases"]]
+        # (an optimizer writes them, so they are copies then; tensor objects of its own, whose .grad is this stack's, in any case)
+        own = optimizer is not None
+        self.w = [t.detach().to(device, copy=own) for t in cfg["weights"]]
+        self.b = [t.detach().to(device, copy=own) for t in cfg["biases"]]
         self.maps = [t.to(device) for t in cfg["maps"]]
         self.reducer = reducer
         self.fuse_relu = fuse_relu
