@@ -246,5 +246,6 @@ class EncoderStack:
         loss = torch.dot(out.reshape(-1), go.reshape(-1))   # sum(out * go) in one pass, without the product tensor
         self.backward(go)
         if self.optimizer is not None:
+            self.parameters()       # (whoever cleared the gradients to None took the buffers away)
             self.optimizer.step()
         return loss

@@ -102,6 +102,18 @@ def test_two_stacks_of_one_config_do_not_share():
         check(b, want[1])
 
 
+@pytest.mark.parametrize("to_none", [False, True])
+def test_cleared_gradients_do_not_end_the_updates(to_none):
+    cfg = config()
+    want = stepped(cfg, 3)
+    with plain_convolutions():
+        stack = stack_of(cfg, optimizer=sgd)
+        for _ in range(3):
+            stack.optimizer.zero_grad(set_to_none=to_none)
+            stack.step(cfg["x"], cfg["grad_output"])
+        check(stack, want)
+
+
 def _rank(rank, world, port, mode, out):
     os.environ["MASTER_ADDR"], os.environ["MASTER_PORT"] = "127.0.0.1", str(port)
     dist.init_process_group("gloo", rank=rank, world_size=world)
@@ -152,6 +164,7 @@ def test_a_config_on_the_device_stays():
     adamw = lambda p: optim.AdamW(p, lr=1e-3)  # noqa: E731
     a, b = (EncoderStack(there, "cuda", 0, 2, optimizer=adamw) for _ in range(2))
     for _ in range(2):
+        a.optimizer.zero_grad()
         a.step(x, go)
     for t, u, v in zip(there["weights"] + there["biases"], cfg["weights"] + cfg["biases"], b.w + b.b):
         assert torch.equal(t.cpu(), u) and torch.equal(v, t) and t.grad is None
