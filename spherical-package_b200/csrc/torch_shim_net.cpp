@@ -50,7 +50,7 @@ void check_device(const Tensor &t, const char *name, const Tensor &like) {
 // How a tensor lies in memory around one of its dimensions.
 struct Layout {
   int64_t dim, outer, C, inner, stride;  // stride of rows (inner == 1)
-  bool moved;                            // rows whose dimension is not the last: outputs are rows seen through movedim
+  bool moved;                            // rows with values behind their dimension too: outputs are rows seen through movedim
 };
 
 Layout layout_of(const Tensor &t, int64_t dim, const char *name) {
@@ -81,8 +81,8 @@ Layout layout_of(const Tensor &t, int64_t dim, const char *name) {
     run = t.stride(i) * t.size(i);
   }
   TORCH_CHECK(rows && step >= l.C, name, " must be contiguous, or rows of one stride with dim of stride 1");
+  l.moved = l.inner > 1;
   l.outer *= l.inner, l.inner = 1, l.stride = step;
-  l.moved = l.dim != t.dim() - 1;
   return l;
 }
 
