@@ -71,6 +71,26 @@ class AdamW(torch.optim.Optimizer):
                 s["master"] = p.detach().float()
         return s
 
+    def _keep_count(self, group, capturing):
+        """The step's number where `capturable` wants it, the group or its params' states, and on from where it was if that has
+        changed since the last step."""
+        if isinstance(group.get("step"), torch.Tensor) if group["capturable"] else "step" not in group:
+            return
+        states = [self.state[p] for p in group["params"] if self.state.get(p)]
+        if not group["capturable"]:
+            n = int(group.pop("step"))
+            for s in states:
+                s["step"] = n
+        else:       # (a number until the device is known)
+            counts = {s["step"] for s in states if "step" in s}
+            if len(counts) > 1:
+                raise RuntimeError("AdamW: params at different step numbers cannot become capturable together")
+            if capturing and states:
+                raise RuntimeError("AdamW: a step has to run before one is captured in a graph")
+            group["step"] = counts.pop() if counts else group.get("step", 0)
+            for s in states:
+                s.pop("step", None)
+
     def load_state_dict(self, state_dict):
         """Moments and masters keep their own types (the base class would cast them to their param's)."""
         super().load_state_dict(state_dict)
@@ -95,6 +115,7 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:
             if capturing and not group["capturable"]:
                 raise RuntimeError("AdamW: a captured step needs capturable=True (its number would stay what it was)")
+            self._keep_count(group, capturing)
             together = {}   # params at one step number: all, unless some had no gradient in an earlier step
             for p in group["params"]:
                 if p.grad is None:
@@ -106,8 +127,8 @@ class AdamW(torch.optim.Optimizer):
             if group["capturable"] and together:
                 if len(together) > 1:
                     raise RuntimeError("a capturable param group must be on one device")
-                if "step" not in group:
-                    group["step"] = torch.zeros((), dtype=torch.float32, device=next(iter(together))[0])
+                if not isinstance(group["step"], torch.Tensor):
+                    group["step"] = torch.tensor(float(group["step"]), device=next(iter(together))[0])
                 group["step"] += 1
             for some in together.values():
                 self._step(group, some)
