@@ -101,8 +101,9 @@ class AdamW(torch.optim.Optimizer):
                 if isinstance(v, torch.Tensor):
                     self.state[p][k] = v.detach().to(device=p.device, copy=True)
         for g in self.param_groups:
-            if isinstance(g.get("step"), torch.Tensor):
-                g["step"] = g["step"].detach().to(device=g["params"][0].device, copy=True)
+            for k in ("step", "lr"):
+                if isinstance(g.get(k), torch.Tensor) and g["params"]:
+                    g[k] = g[k].detach().to(device=g["params"][0].device, copy=True)
 
     @torch.no_grad()
     def step(self, closure=None, grad_scale=1.0):

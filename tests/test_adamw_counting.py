@@ -67,6 +67,19 @@ def test_a_count_is_not_begun_inside_a_graph(calls, monkeypatch):
     assert calls == [1] and "step" not in o.param_groups[0]
 
 
+def test_loading_brings_a_groups_tensors_to_its_device():
+    """Both that a captured step reads, from a checkpoint that was loaded to the host."""
+    def one(device):
+        return optim.AdamW([torch.zeros(4, device=device, requires_grad=True)], lr=torch.tensor(1e-3, device=device), capturable=True)
+    o, other = one("cpu"), one("meta")
+    o.param_groups[0]["step"] = torch.tensor(3.0)
+    o.add_param_group(dict(params=[]))
+    other.add_param_group(dict(params=[]))
+    other.load_state_dict(o.state_dict())
+    group = other.param_groups[0]
+    assert group["step"].device.type == "meta" and group["lr"].device.type == "meta"
+
+
 def test_capturable_groups_count_from_one(calls):
     params, o = optimizer(capturable=True)
     o.step()
