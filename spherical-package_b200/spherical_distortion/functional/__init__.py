@@ -318,7 +318,8 @@ def token_log_probs(logits, target, dim=1, top_k=0, ignore_index=-100):
 
     logits float32, bfloat16 or float16, laid out as for `rms_norm`; target int64, their size without dim.  Results are float32:
     log_probs and entropy of target's size, top_log_probs and (int64) top_indices with top_k in the place of dim, equal
-    logits in the order of their indices; None with top_k = 0.  All but the indices are differentiable.
+    logits in the order of their indices; None with top_k = 0.  All but the indices are differentiable.  More than 32 of the best
+    of rows of more than about 1000 classes cost a pass over the row each, and more than 8 of a pixel's a pass for eight.
 
     A target equal to ignore_index gives log probability 0 and no gradient, any other outside the classes NaN.  Logits of
     -inf are classes out of the question; where there is no other, log probabilities are -inf, the entropy 0 and the
