@@ -426,18 +426,16 @@ class TensorList {
   size_t size_ = 0;
 };
 
-// Whether a step's tensors lie apart in memory.  Those of a list mostly lie one behind the other and the lists apart: then nothing
-// has to be sorted.
-struct Span {
-  uintptr_t from = 0, to = 0;
-  bool written = true;
-};
+// Whether a step's tensors lie apart in memory.  Where those of a list lie one behind the other and the lists apart, nothing has to be
+// sorted.
 struct InOrder {
-  Span list[7];
+  struct {
+    uintptr_t from = 0, to = 0;
+  } list[7];
   bool so = true;
   void next(int k, const void *p, size_t bytes) {
     if (bytes == 0) return;
-    Span &l = list[k];
+    auto &l = list[k];
     if (l.from == l.to) l.from = (uintptr_t)p;
     so = so && (uintptr_t)p >= l.to;
     l.to = (uintptr_t)p + bytes;
@@ -449,17 +447,55 @@ struct InOrder {
     return so;
   }
 };
-// The same of any spans: nothing that is written shares memory with anything else.
-bool apart(std::vector<Span> spans) {
-  std::sort(spans.begin(), spans.end(), [](const Span &a, const Span &b) { return a.from < b.from; });
-  uintptr_t written = 0, read = 0;  // ends of what came so far
-  for (const Span &s : spans) {
-    if (s.from < written || (s.written && s.from < read)) return false;
-    uintptr_t &end = s.written ? written : read;
-    end = std::max(end, s.to);
+// Else what lies forwards or backwards, most of a list as a rule, is merged.
+class Spans {
+ public:
+  explicit Spans(size_t most) { all_.reserve(most); }
+  template <class P> void list(const std::vector<P> &from, const std::vector<int64_t> &numels, size_t bytes, int64_t per, bool written) {
+    const size_t first = all_.size();
+    for (size_t i = 0; i < from.size(); i++)
+      if (numels[i] > 0) all_.push_back({(uintptr_t)from[i], ((uintptr_t)from[i] + bytes * ((numels[i] + per - 1) / per)) << 1 | written});
+    for (auto b = all_.begin() + first; b != all_.end();) {
+      auto e = std::is_sorted_until(b, all_.end());
+      if (e == b + 1) {
+        e = std::is_sorted_until(b, all_.end(), [](const Span &x, const Span &y) { return y < x; });
+        std::reverse(b, e);
+      }
+      ends_.push_back(e - all_.begin());
+      b = e;
+    }
   }
-  return true;
-}
+  // Whether nothing that is written shares memory with anything else.
+  bool apart() {
+    std::vector<Span> other(all_.size());
+    while (ends_.size() > 1) {
+      std::vector<size_t> ends;
+      size_t at = 0;
+      for (size_t k = 0; k < ends_.size(); k += 2) {
+        const size_t mid = ends_[k], end = k + 1 < ends_.size() ? ends_[k + 1] : mid;
+        std::merge(all_.begin() + at, all_.begin() + mid, all_.begin() + mid, all_.begin() + end, other.begin() + at);
+        ends.push_back(at = end);
+      }
+      all_.swap(other), ends_.swap(ends);
+    }
+    uintptr_t written = 0, read = 0;  // ends of what came so far
+    for (const Span &s : all_) {
+      const bool w = s.to_written & 1;
+      if (s.from < written || (w && s.from < read)) return false;
+      uintptr_t &end = w ? written : read;
+      end = std::max(end, s.to_written >> 1);
+    }
+    return true;
+  }
+
+ private:
+  struct Span {
+    uintptr_t from, to_written;  // (the end, and whether it is written in the lowest bit)
+    bool operator<(const Span &o) const { return from < o.from; }
+  };
+  std::vector<Span> all_;
+  std::vector<size_t> ends_;
+};
 
 void adamw_step(const py::object &params_list, const py::object &grads_list, const py::object &m_list, const py::object &v_list,
                 const py::object &masters_list, const py::object &m_scales_list, const py::object &v_scales_list, double step, double lr,
@@ -544,14 +580,18 @@ void adamw_step(const py::object &params_list, const py::object &grads_list, con
   const c10::Device device = like.device();
   const TensorList *lists[] = {&params, &grads, &m, &v, &masters, &m_scales, &v_scales};
   if (!order.apart()) {
-    std::vector<Span> spans;
-    for (const TensorList *list : lists)
-      for (size_t i = 0; *list && i < n; i++)
-        if (list->has(i) && (*list)[i].numel() > 0) {
-          const uintptr_t from = (uintptr_t)(*list)[i].unsafeGetTensorImpl()->data();
-          spans.push_back({from, from + (*list)[i].nbytes(), list != &grads});
-        }
-    TORCH_CHECK(apart(std::move(spans)), "adamw_step: a tensor that is written appears twice, or overlaps another");
+    Spans spans(7 * n);
+    for (const Group &q : groups) {
+      const size_t state_bytes = eight ? 1 : 4;
+      spans.list(q.p, q.n, element_bytes(q.dtype), 1, true);
+      spans.list(q.g, q.n, element_bytes(q.grad_dtype), 1, false);
+      spans.list(q.m, q.n, state_bytes, 1, true);
+      spans.list(q.v, q.n, state_bytes, 1, true);
+      spans.list(q.w, q.n, 4, 1, true);
+      spans.list(q.ms, q.n, 4, 256, true);
+      spans.list(q.vs, q.n, 4, 256, true);
+    }
+    TORCH_CHECK(spans.apart(), "adamw_step: a tensor that is written appears twice, or overlaps another");
   }
   for (const TensorList *list : lists)
     for (size_t i = 0; *list && i < n; i++)

@@ -1,4 +1,6 @@
 """Calls of the AdamW step that would be lost or go wrong without a word, refused before any device is asked for."""
+import random
+
 import pytest
 import torch
 
@@ -78,3 +80,27 @@ def test_what_does_not_overlap_is_not_refused_for_it():
         b[name] = [row[:300], row[300:]]
     with pytest.raises(RuntimeError, match="CUDA tensor"):
         step(b)
+
+
+def test_overlaps_at_random():
+    """Against a look at all pairs: tensors anywhere in one allocation, in any order, of which a few or none overlap."""
+    rng = random.Random(5)
+    found = [0, 0]
+    for _ in range(400):
+        n, one = rng.randrange(1, 12), torch.zeros(1 << 14)
+        starts = rng.sample(range(0, 1 << 14, 64), 4 * n)
+        if rng.random() < 0.5:
+            starts.sort(reverse=rng.random() < 0.5)
+        a, spans = dict(params=[], grads=[], exp_avgs=[], exp_avg_sqs=[]), []
+        for i in range(n):
+            size = rng.choice((0, 1, 63, 64, 64, rng.choice((64, 65))))
+            for k, name in enumerate(a):
+                at = min(starts[4 * i + k], (1 << 14) - size)
+                a[name].append(one[at:at + size])
+                if size:
+                    spans.append((at, at + size, name != "grads"))
+        clash = any((p[2] or q[2]) and p[0] < q[1] and q[0] < p[1] for i, p in enumerate(spans) for q in spans[:i])
+        found[clash] += 1
+        with pytest.raises(RuntimeError, match="overlaps" if clash else "CUDA tensor"):
+            step(a)
+    assert min(found) > 40
